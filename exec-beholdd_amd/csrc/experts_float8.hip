@@ -1,0 +1,286 @@
+// Routed experts whose matrices are kept in 8 bits (float8.h): for every (row, choice) pair p = row * top + j and its expert e = chosen[p]
+//   inner[p] = act(Wg_e x[row], Wu_e x[row])     act(g, u) = g' / (1 + exp(-alpha g')) * (u' + shift), g' = min(g, limit), u' = clamp(u, +-limit)
+//   y[p]     = Wd_e inner[p]                     inner in 32 bits, brought into 8 once
+//   out[row] (+)= sum over j of weight[p] * y[p], j in order
+// A pair's weight may multiply the expert's input instead (its gate and up sums).  A pair whose expert is none of the E gives nothing, or,
+// with `through`, one numbered E or higher hands the row's input on.  Nothing here depends on the routing on the host.
+//   few    an expert's pairs 16 at a time, quantised by the waves that multiply them (gemm_float8.hip's product of few rows)
+//   tiles  tiles of 64 pairs of an expert from rows in 8 bits, found from the experts' counts by every workgroup itself
+#include "float8_few.h"
+#include "float8_tiles.h"
+
+namespace {
+
+struct ExpertGate {
+  float limit, alpha, shift;
+};
+__device__ inline float activated(float g, float u, const ExpertGate& gate) {
+  g = fminf(g, gate.limit);
+  u = fminf(fmaxf(u, -gate.limit), gate.limit);
+  return g / (1.0f + expf(-gate.alpha * g)) * (u + gate.shift);
+}
+
+// ---- few -------------------------------------------------------------------------------------------------------
+constexpr int FEW_WAVES = 8, FEW_PAIRS = 4096;      // pairs of a call at most
+
+// grid (blocks of 16 outputs, min(pairs, E)).  With at most E pairs a workgroup is a pair's, and the first pair of an expert does all of
+// that expert's; otherwise it is an expert's.  The list of the expert's pairs is made here, by a wave, in their order.
+template <typename T, bool GATED, bool FULL, bool WHOLE>
+__global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __restrict__ in, int in_div, const int32_t* __restrict__ chosen, int pairs,
+                                                                    int E, F8Weight w, float* __restrict__ out, int K, ExpertGate gate,
+                                                                    const float* __restrict__ in_weights) {
+  constexpr int TT = GATED ? 2 : 1;
+  __shared__ float partial[FEW_WAVES][TT][256];
+  __shared__ int mine[FEW_PAIRS];
+  __shared__ int found;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, i = lane % 16, q = lane / 16;
+  const int expert = pairs <= E ? chosen[blockIdx.y] : (int)blockIdx.y;
+  if (expert < 0 || expert >= E) return;      // the whole workgroup
+  if (wave == 0) {
+    int count = 0;
+    for (int p0 = 0; p0 < pairs; p0 += 64) {
+      const bool is = p0 + lane < pairs && chosen[min(p0 + lane, pairs - 1)] == expert;
+      const unsigned long long mask = __ballot(is);
+      if (is) mine[count + __popcll(mask & ((1ull << lane) - 1ull))] = p0 + lane;
+      count += __popcll(mask);
+    }
+    if (lane == 0) found = count;
+  }
+  __syncthreads();
+  const int count = found;
+  if (count == 0 || (pairs <= E && mine[0] != (int)blockIdx.y)) return;
+  const int block = blockIdx.x, blocks = w.blocks(), stretches = w.stretches;
+  const uint8_t* wp[TT];
+  const float* ws[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const long matrix = (long)expert * TT + t;
+    wp[t] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    ws[t] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+  }
+  for (int p0 = 0; p0 < count; p0 += 16) {
+    const bool there = p0 + i < count;
+    const T* row = in + (size_t)(mine[min(p0 + i, count - 1)] / in_div) * K;
+    f8_f32x4_t acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
+    f8_u32x4_t wv[2][TT][2];
+    float wsv[2][TT];
+    F8Stretch<T> xv[2];
+    auto ask = [&](int u, int j) {
+      f8_load_stretch<T, WHOLE>(xv[u], row, there, j * F8_K + 16 * q, K);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
+        wv[u][t][0] = from[0], wv[u][t][1] = from[64];
+        wsv[u][t] = ws[t][j];
+      }
+    };
+    auto multiply = [&](int u) {
+      F8Operand<FULL> xo;
+      float xs;
+      xo.set(xv[u].quantised(&xs));
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        F8Operand<FULL> wo;
+        wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
+        const f8_f32x4_t sum = f8_stretch(wo, xo);
+        const float s = xs * wsv[u][t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sum[e], s, acc[t][e]);
+      }
+    };
+    int j = wave;
+    if (j < stretches) ask(0, j);
+    for (; j < stretches; j += 2 * FEW_WAVES) {
+      if (j + FEW_WAVES < stretches) ask(1, j + FEW_WAVES);
+      multiply(0);
+      if (j + 2 * FEW_WAVES < stretches) ask(0, j + 2 * FEW_WAVES);
+      if (j + FEW_WAVES < stretches) multiply(1);
+    }
+    if (p0) __syncthreads();      // the sums of the pairs before have been read
+#pragma unroll
+    for (int t = 0; t < TT; ++t) *reinterpret_cast<f8_f32x4_t*>(&partial[wave][t][i * 16 + 4 * q]) = acc[t];
+    __syncthreads();
+    const int e = threadIdx.x, m = e / 16, n = block * 16 + e % 16;
+    if (e < 256 && p0 + m < count && n < w.rows) {
+      const int pair = mine[p0 + m];
+      float sum[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        sum[t] = 0.f;
+#pragma unroll
+        for (int v = 0; v < FEW_WAVES; ++v) sum[t] += partial[v][t][e];
+      }
+      if constexpr (GATED) {
+        const float wgt = in_weights ? in_weights[pair] : 1.0f;
+        out[(size_t)pair * w.rows + n] = activated(sum[0] * wgt, sum[TT - 1] * wgt, gate);
+      } else {
+        out[(size_t)pair * w.rows + n] = sum[0];
+      }
+    }
+  }
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------------------
+// a: rows in 8 bits, row after row; the input of pair p is row p / in_div.
+template <bool GATED, bool FULL>
+__global__ __launch_bounds__(256) void experts_tiles8_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded, int in_div,
+                                                             const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
+                                                             F8Weight w, float* __restrict__ out, ExpertGate gate, const float* __restrict__ in_weights) {
+  constexpr int XB = 2, YB = 4, ROWS = 64, OUTS = GATED ? 64 : 128, HALF = GATED ? YB / 2 : YB;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 2, wn = wave % 2;
+  const int n_tiles = (w.rows + OUTS - 1) / OUTS, stretches = w.stretches, blocks = w.blocks();
+  // the expert and the tile of pairs: a wave adds up 64 experts' tiles at a time; every wave of the workgroup finds the same
+  int expert = -1, before = 0, count = 0, at = 0;
+  for (int e0 = 0; e0 < E && expert < 0; e0 += 64) {
+    const int own = e0 + lane < E ? counts[e0 + lane] : 0, tiles = (own + ROWS - 1) / ROWS * n_tiles;
+    int upto = tiles;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int lower = __shfl_up(upto, off, BH_WAVE);
+      if (lane >= off) upto += lower;
+    }
+    const unsigned long long behind = __ballot(before + upto > (int)blockIdx.x);
+    if (behind) {
+      const int l = __ffsll(behind) - 1;
+      expert = e0 + l;
+      count = __shfl(own, l, BH_WAVE);
+      at = (int)blockIdx.x - before - (__shfl(upto, l, BH_WAVE) - __shfl(tiles, l, BH_WAVE));
+    } else {
+      before += __shfl(upto, 63, BH_WAVE);
+    }
+  }
+  if (expert < 0) return;      // beyond the last tile: the whole workgroup
+  expert = __builtin_amdgcn_readfirstlane(expert);
+  count = __builtin_amdgcn_readfirstlane(count);
+  at = __builtin_amdgcn_readfirstlane(at);
+  const int row_tiles = (count + ROWS - 1) / ROWS, p0 = (at % row_tiles) * ROWS, tile_n = at / row_tiles;
+  const int32_t* pairs = list + (size_t)expert * capacity;
+  const uint8_t* ap[XB];
+  const uint8_t* wp[YB];
+  const float* ws[YB];
+  const uint32_t* xp[XB];
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    const int row = pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)] / in_div;
+    ap[x] = a + (size_t)row * stretches * F8_K + 16 * (lane / 16);
+    xp[x] = exponents + row;
+  }
+#pragma unroll
+  for (int y = 0; y < YB; ++y) {
+    const int block = min((tile_n * 2 + wn) * HALF + y % HALF, blocks - 1);
+    const long matrix = (long)expert * (GATED ? 2 : 1) + y / HALF;
+    wp[y] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    ws[y] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+  }
+  f8_f32x4_t acc[XB][YB];
+#pragma unroll
+  for (int x = 0; x < XB; ++x)
+#pragma unroll
+    for (int y = 0; y < YB; ++y) acc[x][y] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f8_walk<FULL, XB, YB, F8_K, 64>(ap, xp, padded, wp, ws, 0, stretches, acc);
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    const int p = p0 + (wm * XB + x) * 16 + lane % 16;
+    if (p >= count) continue;
+    const int pair = pairs[p];
+    const float wgt = GATED && in_weights ? in_weights[pair] : 1.0f;
+#pragma unroll
+    for (int y = 0; y < HALF; ++y) {
+      const int n = ((tile_n * 2 + wn) * HALF + y) * 16 + 4 * (lane / 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= w.rows) break;
+        out[(size_t)pair * w.rows + n + e] =
+            GATED ? activated(acc[x][y][e] * wgt, acc[x][y + (GATED ? HALF : 0)][e] * wgt, gate) : acc[x][y][e];
+      }
+    }
+  }
+}
+
+// ---- the sum over a row's pairs --------------------------------------------------------------------------------
+template <typename T, typename TC>
+__global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restrict__ y, const int32_t* __restrict__ chosen, const float* __restrict__ weights,
+                                                          const T* __restrict__ through, TC* __restrict__ out, int E, int top, int D, int fresh) {
+  const int row = blockIdx.x, d = blockIdx.y * blockDim.x + threadIdx.x;
+  if (d >= D) return;
+  float total = 0.f;
+  for (int j = 0; j < top; ++j) {
+    const long pair = (long)row * top + j;
+    const int e = chosen[pair];
+    if (e < 0 || (e >= E && through == nullptr)) continue;
+    const float share = e >= E ? to_f32(through[(size_t)row * D + d]) : y[pair * D + d];
+    total = fmaf(weights ? weights[pair] : 1.0f, share, total);
+  }
+  TC* at = out + (size_t)row * D + d;
+  *at = from_f32<TC>(fresh ? total : to_f32(*at) + total);
+}
+
+}  // namespace
+
+// Whether the pairs of a call go through `few`.
+extern "C" int bh_experts_float8_few(int pairs, int E) { return pairs <= FEW_PAIRS && pairs <= 8 * E; }
+
+// One of the two products of `few`: in [*][K] rows of `dtype`; out float32 [pairs][N]; gated: w holds gate and up of every expert.
+extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, const int32_t* chosen, int pairs, int E, const void* w, const void* scales,
+                                      float* out, int N, int K, int gated, float limit, float alpha, float shift, const float* in_weights, int full,
+                                      hipStream_t stream) {
+  BH_REQUIRE(pairs > 0 && pairs <= FEW_PAIRS && E > 0 && N > 0 && K > 0 && in_div > 0, "experts_float8: 1 to %d pairs of positive sizes, got %d", FEW_PAIRS, pairs);
+  BH_REQUIRE((uintptr_t)w % 16 == 0, "experts_float8: the weights must be 16-byte aligned");
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+  const dim3 grid(weight.blocks(), pairs < E ? pairs : E);
+  BH_REQUIRE(grid.y <= 65535, "experts_float8: up to 65,535 experts");
+  const bool whole = K % 8 == 0 && (uintptr_t)in % 16 == 0;
+  const ExpertGate gate = {limit, alpha, shift};
+#define BH_F8_EXPERTS(T, GATED, FULL)                                                                                                                   \
+  do {                                                                                                                                                  \
+    if (whole) experts_few_kernel<T, GATED, FULL, true><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights); \
+    else experts_few_kernel<T, GATED, FULL, false><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights);      \
+  } while (0)
+#define BH_F8_EXPERTS_OF(T)                                                                                \
+  do {                                                                                                     \
+    if (gated) { if (full) BH_F8_EXPERTS(T, true, true); else BH_F8_EXPERTS(T, true, false); }             \
+    else { if (full) BH_F8_EXPERTS(T, false, true); else BH_F8_EXPERTS(T, false, false); }                 \
+  } while (0)
+  if (dtype == BH_F32) BH_F8_EXPERTS_OF(float);
+  else if (dtype == BH_BF16) BH_F8_EXPERTS_OF(bf16_t);
+  else return bh_fail("experts_float8: unknown dtype %d", dtype);
+  return bh_check_launch("experts_float8_rows");
+}
+
+// One of the two products of `tiles`, from rows in 8 bits; lists [E][capacity] and counts [E] as experts_group makes them.
+extern "C" int bh_experts_float8_tiles(const void* a, const void* exponents, int rows, int in_div, const int32_t* list, int capacity, const int32_t* counts,
+                                       int pairs, int E, const void* w, const void* scales, float* out, int N, int K, int gated, float limit, float alpha,
+                                       float shift, const float* in_weights, int full, hipStream_t stream) {
+  BH_REQUIRE(rows > 0 && pairs > 0 && E > 0 && N > 0 && K > 0 && in_div > 0 && capacity > 0, "experts_float8: sizes must be positive");
+  BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents | (uintptr_t)w) % 16 == 0, "experts_float8: rows and weights must be 16-byte aligned");
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+  const int outs = gated ? 64 : 128;
+  const long most = (long)((N + outs - 1) / outs) * (pairs / 64 + (pairs < E ? pairs : E));      // every expert's last tile may be a part of one
+  BH_REQUIRE(most < (1L << 31), "experts_float8: %d pairs of %d outputs are too many", pairs, N);
+  const ExpertGate gate = {limit, alpha, shift};
+#define BH_F8_TILES(GATED, FULL)                                                                                                                \
+  experts_tiles8_kernel<GATED, FULL><<<(unsigned)most, 256, 0, stream>>>((const uint8_t*)a, (const uint32_t*)exponents, (rows + 15) / 16 * 16, in_div, \
+                                                                        list, capacity, counts, E, weight, out, gate, in_weights)
+  if (gated) {
+    if (full) BH_F8_TILES(true, true);
+    else BH_F8_TILES(true, false);
+  } else if (full) BH_F8_TILES(false, true);
+  else BH_F8_TILES(false, false);
+  return bh_check_launch("experts_float8_tiles");
+}
+
+extern "C" int bh_experts_float8_sum(const float* y, const int32_t* chosen, const float* weights, const void* through, int dtype, void* out, int c_dtype,
+                                     int n_rows, int E, int top, int D, int fresh, hipStream_t stream) {
+  BH_REQUIRE(n_rows > 0 && top > 0 && D > 0 && E > 0 && (D + 255) / 256 <= 65535, "experts_float8: %d rows of %d outputs", n_rows, D);
+  const dim3 grid(n_rows, (D + 255) / 256);
+#define BH_F8_SUM(T, TC) experts_sum_kernel<T, TC><<<grid, 256, 0, stream>>>(y, chosen, weights, (const T*)through, (TC*)out, E, top, D, fresh)
+  BH_REQUIRE((dtype == BH_F32 || dtype == BH_BF16) && (c_dtype == BH_F32 || c_dtype == BH_BF16), "experts_float8: unknown dtype");
+  if (dtype == BH_F32) {
+    if (c_dtype == BH_F32) BH_F8_SUM(float, float);
+    else BH_F8_SUM(float, bf16_t);
+  } else if (c_dtype == BH_F32) BH_F8_SUM(bf16_t, float);
+  else BH_F8_SUM(bf16_t, bf16_t);
+  return bh_check_launch("experts_float8_sum");
+}

@@ -1,0 +1,114 @@
+// Products with weights and activations in 8-bit floating point (e4m3, its largest value 448): layouts and device code that the kernels
+// of float8_rows.hip, gemm_float8.hip and experts_float8.hip share.
+//
+// Weights [rows][K]: blocks of 16 rows x 128 k, 2 KB each, along k first, in operand order (f8_place); rows and k beyond the matrix are
+// zeros.  A scale (float32) for each 128 rows x 128 k, [ceil(rows / 128)][ceil(K / 128)].  Several matrices of as many rows lie one behind
+// the other, each with whole blocks of its own.
+// Activations: the same blocks, of rows of activations.  A stretch of 128 k of a row has the scale 2^e with the least e >= -126 for which
+// no value exceeds 448 * 2^e: dividing by it is exact, so that a value is rounded once, and two kernels that quantise the same row give
+// the same bytes.  Kept as the exponent's byte e + 127, four stretches in a word: word [k / 512][row], byte (k / 128) % 4.  An infinity or
+// a NaN becomes e4m3's NaN, so that every output of its row is NaN.
+//
+// y[r][n] = sum over stretches j of (sum over k in j of q[r][k] w[n][k]) * (scale of the row's stretch * scale of the weights' block):
+// the inner sum is one v_mfma_f32_16x16x128 of a stretch, the outer one float32 fused multiply-adds.
+//
+// What the matrix cores add up: the 8-bit MFMA aligns the products of 8 neighbouring k to the largest of them and drops what lies 2^14
+// below it (a measured 1.4e-5 of the sum, as the norm of the error over that of the sums, for normally distributed values), then adds in
+// float32.  An output rounded to bfloat16 (2^-9 on average) does not show it.  Where the output is float32 the kernels are compiled FULL:
+// the operands are widened to bfloat16, which holds every e4m3 value, and go through the bfloat16 MFMA at half the rate, whose products
+// and sums are those of float32 (9e-9 measured).
+#pragma once
+#include "common.h"
+
+#define F8_K 128            // k of a stretch, and of an MFMA
+#define F8_BLOCK 2048       // bytes of 16 rows x 128 k
+
+typedef int f8_operand_t __attribute__((ext_vector_type(8)));
+typedef float f8_f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t f8_u32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 f8_bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 f8_bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short f8_s16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t f8_u16x2_t __attribute__((ext_vector_type(2)));
+
+// Byte of (row, k) within a block: lane 16 q + row of an operand holds k 16 q .. + 15 (half 0) and 64 + 16 q .. + 15 (half 1), so that
+// either half of an operand is 1 KB of neighbouring bytes, and 64 neighbouring bytes of each row.
+BH_BOTH inline int f8_place(int row, int k) { return (k / 64) * 1024 + ((k % 64) / 16 * 16 + row) * 16 + k % 16; }
+
+// The exponent's byte of a stretch whose largest magnitude has these float32 bits: 448 = 1.75 * 2^8.
+__device__ inline uint32_t f8_exponent(uint32_t largest) {
+  const int e = (int)(largest >> 23) - 8 + ((largest & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(e, 1);
+}
+__device__ inline float f8_scale(uint32_t exponent) { return __builtin_bit_cast(float, exponent << 23); }
+
+// Four values as bytes of a word.
+__device__ inline uint32_t f8_four(float a, float b, float c, float d, float scale) {
+  f8_s16x2_t v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, a, b, scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(v, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, v);
+}
+// The same of two words of bfloat16.
+__device__ inline uint32_t f8_four(uint32_t ab, uint32_t cd, float scale) {
+  f8_s16x2_t v = {0, 0};
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(f8_bf16x2_t, ab), scale, false);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(f8_bf16x2_t, cd), scale, true);
+  return __builtin_bit_cast(uint32_t, v);
+}
+// The largest magnitude so far, float32 bits (a NaN is larger than infinity so).
+__device__ inline uint32_t f8_larger(uint32_t largest, float v) { return max(largest, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu); }
+// The same for two halves of bfloat16 at once, 16 bits each.
+__device__ inline uint32_t f8_larger_pair(uint32_t largest, uint32_t pair) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(f8_u16x2_t, largest), __builtin_bit_cast(f8_u16x2_t, pair & 0x7fff7fffu)));
+}
+__device__ inline uint32_t f8_of_pair(uint32_t pair) { return max(pair & 0xffffu, pair >> 16) << 16; }
+
+// A block's operand as it lies: a lane's two halves of 16 bytes.
+__device__ inline f8_operand_t f8_operand(f8_u32x4_t a, f8_u32x4_t b) {
+  return f8_operand_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+// 8 values of an operand (two of its words) widened.
+__device__ inline f8_bf16x8_t f8_widen(int first, int second) {
+  const f8_bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(first, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(first, 1.0f, true);
+  const f8_bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(second, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(second, 1.0f, true);
+  return f8_bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// An operand, widened once where the sums are full.
+template <bool FULL>
+struct F8Operand {
+  f8_operand_t v;
+  __device__ inline void set(f8_operand_t from) { v = from; }
+};
+template <>
+struct F8Operand<true> {
+  f8_bf16x8_t v[4];
+  __device__ inline void set(f8_operand_t from) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f8_widen(from[2 * i], from[2 * i + 1]);
+  }
+};
+// A stretch's sums: rows of `w` x rows of `x`; a lane holds rows 4 (lane / 16) .. + 3 of w for row lane % 16 of x.
+__device__ inline f8_f32x4_t f8_stretch(const F8Operand<false>& w, const F8Operand<false>& x) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f8_f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ inline f8_f32x4_t f8_stretch(const F8Operand<true>& w, const F8Operand<true>& x) {
+  f8_f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], x.v[i], sum, 0, 0, 0);
+  return sum;
+}
+
+// A weight of `matrices` matrices [rows][K] as the kernels see it.
+struct F8Weight {
+  const uint8_t* data;
+  const float* scales;
+  int rows, stretches;      // of one matrix: its rows, ceil(K / 128)
+  __host__ __device__ int blocks() const { return (rows + 15) / 16; }
+  __host__ __device__ int scale_rows() const { return (rows + F8_K - 1) / F8_K; }
+};
+
+// ---- what the sources tell each other ------------------------------------------------------------------------
+// Activation rows [rows][width] (bfloat16 or float32, row after row) in 8 bits: `data` whole blocks, `exponents` [ceil(width / 512)][padded
+// rows] words, rows padded to 16.  in_rows: `data` row after row, each of whole stretches.  gate 0: as they are; else a row holds 2 * width values, gate then up, and act(gate) * up is quantised.
+int float8_rows_launch(const void* x, int dtype, uint8_t* data, uint32_t* exponents, int rows, int width, int in_rows, int gate, hipStream_t stream);

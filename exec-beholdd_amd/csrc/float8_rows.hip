@@ -1,0 +1,99 @@
+// Activation rows in 8 bits (float8.h): one pass over the rows, which it is bound by reading.
+//   float8_rows   [rows][width] bfloat16 or float32 -> blocks of 16 rows x 128 k of e4m3 and a word of exponents for each 512 k of a row;
+//                 of rows [gate | up] the activation act(gate) * up, in 32 bits until it is rounded once
+//
+// 16 lanes hold a stretch of 128 values, 8 each (16 bytes of bfloat16), a wave four stretches of a row: its largest magnitude takes four
+// steps between lanes, the exponents of the four stretches make one word.  A workgroup of four waves takes the 16 rows of a block, four a
+// wave one after the other, so that the 256-byte runs of a block that its rows write in pieces of 8 bytes meet in one L2.
+#include "float8.h"
+
+namespace {
+
+// 8 neighbouring values of a row from `k` on, zeros beyond its width.  WHOLE: they are all there, on an address of 16 bytes.
+template <typename T, bool WHOLE>
+__device__ inline void load_eight(const T* __restrict__ row, int k, int width, float v[8]) {
+  if constexpr (WHOLE) {
+    if (k < width) {
+      const float4 a = load_four(row + k), b = load_four(row + k + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < width ? to_f32(row[k + i]) : 0.f;
+  }
+}
+
+// grid (ceil(rows / 16), ceil(width / 512)).
+// `in_rows`: row after row instead, each of whole stretches (what the experts' products pick their rows from).
+template <typename T, bool GATED, bool WHOLE>
+__global__ __launch_bounds__(256) void float8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ data, uint32_t* __restrict__ exponents,
+                                                          int rows, int width, int in_rows, GateForm form) {
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int stretches = (width + F8_K - 1) / F8_K, k = blockIdx.y * 512 + lane * 8, stretch = k / F8_K;
+  const int padded = (rows + 15) / 16 * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = wave * 4 + i;
+    const long row = (long)blockIdx.x * 16 + r;
+    if (row >= rows) break;
+    const T* from = x + row * (GATED ? 2L * width : (long)width);
+    float v[8];
+    load_eight<T, WHOLE>(from, k, width, v);
+    if constexpr (GATED) {
+      float u[8];
+      load_eight<T, WHOLE>(from + width, k, width, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = gate_mul(v[j], u[j], form);
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) largest = f8_larger(largest, v[j]);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, off, BH_WAVE));
+    const uint32_t exponent = f8_exponent(largest);
+    const float scale = f8_scale(exponent);
+    if (stretch < stretches) {
+      const uint2 eight = make_uint2(f8_four(v[0], v[1], v[2], v[3], scale), f8_four(v[4], v[5], v[6], v[7], scale));
+      const long at = in_rows ? (row * stretches + stretch) * F8_K + k % F8_K
+                              : ((long)blockIdx.x * stretches + stretch) * F8_BLOCK + f8_place(r, k % F8_K);
+      *reinterpret_cast<uint2*>(data + at) = eight;
+    }
+    uint32_t word = exponent << (8 * (lane / 16));
+    word |= (uint32_t)__shfl_xor((int)word, 16, BH_WAVE);
+    word |= (uint32_t)__shfl_xor((int)word, 32, BH_WAVE);
+    if (lane == 0) exponents[(long)blockIdx.y * padded + row] = word;
+  }
+}
+
+template <typename T>
+void launch(const void* x, uint8_t* data, uint32_t* exponents, int rows, int width, int in_rows, int gate, hipStream_t stream) {
+  const dim3 grid((rows + 15) / 16, (width + 511) / 512);
+  const bool whole = width % 8 == 0 && (uintptr_t)x % 16 == 0;
+  const GateForm form = bh_gate_form(gate);
+#define BH_F8_ROWS(GATED, WHOLE) float8_rows_kernel<T, GATED, WHOLE><<<grid, 256, 0, stream>>>((const T*)x, data, exponents, rows, width, in_rows, form)
+  if (gate) {
+    if (whole) BH_F8_ROWS(true, true);
+    else BH_F8_ROWS(true, false);
+  } else if (whole) BH_F8_ROWS(false, true);
+  else BH_F8_ROWS(false, false);
+#undef BH_F8_ROWS
+}
+
+}  // namespace
+
+int float8_rows_launch(const void* x, int dtype, uint8_t* data, uint32_t* exponents, int rows, int width, int in_rows, int gate, hipStream_t stream) {
+  BH_REQUIRE(rows > 0 && width > 0 && width <= (1 << 24), "float8_rows: %d rows of %d values", rows, width);
+  BH_REQUIRE(gate == 0 || gate == BH_GATE_SILU || gate == BH_GATE_GELU_TANH, "float8_rows: unknown gate %d", gate);
+  BH_REQUIRE(((uintptr_t)data | (uintptr_t)exponents) % 16 == 0, "float8_rows: the 8-bit rows must be 16-byte aligned");
+  if (dtype == BH_F32) launch<float>(x, data, exponents, rows, width, in_rows, gate, stream);
+  else if (dtype == BH_BF16) launch<bf16_t>(x, data, exponents, rows, width, in_rows, gate, stream);
+  else return bh_fail("float8_rows: unknown dtype %d", dtype);
+  return bh_check_launch("float8_rows");
+}
+
+extern "C" int bh_float8_rows(const void* x, int dtype, void* data, void* exponents, int rows, int width, int in_rows, int gate, hipStream_t stream) {
+  return float8_rows_launch(x, dtype, (uint8_t*)data, (uint32_t*)exponents, rows, width, in_rows, gate, stream);
+}

@@ -1,0 +1,277 @@
+// Matrix products with weights and activations in 8 bits (float8.h): C[M, N] (+)= x[M, K] * W[N, K]^T, plain or gated.
+//   few     up to 32 rows, straight from bfloat16 or float32 rows: a wave quantises the stretch it multiplies
+//   tiles   any number of rows, from rows in 8 bits (float8_rows.hip), K in parts where the tiles alone leave compute units idle
+#include "float8_few.h"
+#include "float8_tiles.h"
+
+namespace {
+
+// ---- a few rows ------------------------------------------------------------------------------------------------
+// Bound by reading W once.  A workgroup owns NT blocks of 16 weight rows (gated: as many pairs of gate and up); its eight waves take the
+// stretches of k in turn, each with the next one on its way, and quantise the rows' stretch themselves: 16 values a lane and half an
+// operand, the largest of a stretch found between the four lanes of a row.  The waves' sums are added through LDS in a fixed order.
+constexpr int FEW_WAVES = 8;
+
+// grid (ceil(blocks of W / NT)).  MB: blocks of 16 rows.  TC: the output's type.
+template <typename T, typename TC, int MB, int NT, bool GATED, bool FULL, bool WHOLE>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict__ x, F8Weight w, TC* __restrict__ c, int M, int K, int ldc,
+                                                             int accumulate, GateForm form) {
+  constexpr int TT = NT * (GATED ? 2 : 1);
+  __shared__ float partial[FEW_WAVES][TT][MB][256];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int i = lane % 16, q = lane / 16, blocks = w.blocks(), stretches = w.stretches;
+  const uint8_t* wp[TT];
+  const float* ws[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int block = min((int)blockIdx.x * NT + t % NT, blocks - 1);      // (one beyond the last repeats it and stores nothing)
+    const int matrix = t / NT;
+    wp[t] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    ws[t] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+  }
+  f8_f32x4_t acc[TT][MB];
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[t][b] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f8_u32x4_t wv[2][TT][2];
+  float wsv[2][TT];
+  F8Stretch<T> xv[2][MB];
+  auto ask = [&](int u, int j) {
+#pragma unroll
+    for (int b = 0; b < MB; ++b) f8_load_stretch<T, WHOLE>(xv[u][b], x + (size_t)min(b * 16 + i, M - 1) * K, b * 16 + i < M, j * F8_K + 16 * q, K);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
+      wv[u][t][0] = __builtin_nontemporal_load(from);
+      wv[u][t][1] = __builtin_nontemporal_load(from + 64);
+      wsv[u][t] = ws[t][j];
+    }
+  };
+  auto multiply = [&](int u) {
+    F8Operand<FULL> xo[MB];
+    float xs[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) xo[b].set(xv[u][b].quantised(&xs[b]));
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      F8Operand<FULL> wo;
+      wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        const f8_f32x4_t sum = f8_stretch(wo, xo[b]);
+        const float s = xs[b] * wsv[u][t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][b][e] = fmaf(sum[e], s, acc[t][b][e]);
+      }
+    }
+  };
+  int j = wave;
+  if (j < stretches) ask(0, j);
+  for (; j < stretches; j += 2 * FEW_WAVES) {
+    if (j + FEW_WAVES < stretches) ask(1, j + FEW_WAVES);
+    multiply(0);
+    if (j + 2 * FEW_WAVES < stretches) ask(0, j + 2 * FEW_WAVES);
+    if (j + FEW_WAVES < stretches) multiply(1);
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int b = 0; b < MB; ++b) *reinterpret_cast<f8_f32x4_t*>(&partial[wave][t][b][i * 16 + 4 * q]) = acc[t][b];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MB * 256; e += FEW_WAVES * 64) {
+    const int b = e / 256, m = b * 16 + (e % 256) / 16, column = e % 16;
+    if (m >= M) continue;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = ((int)blockIdx.x * NT + t) * 16 + column;
+      if (n >= w.rows) continue;
+      float sum[GATED ? 2 : 1];
+#pragma unroll
+      for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+        sum[g] = 0.f;
+#pragma unroll
+        for (int v = 0; v < FEW_WAVES; ++v) sum[g] += partial[v][g * NT + t][b][e % 256];
+      }
+      TC* at = c + (size_t)m * ldc + n;
+      float value = GATED ? gate_mul(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
+      if (accumulate) value += to_f32(*at);
+      *at = from_f32<TC>(value);
+    }
+  }
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------------------
+// Four waves of 32 rows x 64 weight rows each, operands straight from memory, the next stretch's on their way.
+// With K in parts (grid y) part p leaves its bare sums at sums + p * M * width, width = N, or 2 N of a gated product (gate, then up).
+template <typename TC, bool GATED, bool FULL, bool PARTS>
+__global__ __launch_bounds__(256) void tiles_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, F8Weight w,
+                                                    TC* __restrict__ c, int M, int ldc, int accumulate, GateForm form) {
+  constexpr int XB = 2, YB = 4, OUTS = GATED ? 64 : 128, HALF = GATED ? YB / 2 : YB;      // a wave's blocks of outputs
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 2, wn = wave % 2;
+  const int n_tiles = (w.rows + OUTS - 1) / OUTS, tile_n = blockIdx.x % n_tiles, tile_m = blockIdx.x / n_tiles;
+  const int stretches = w.stretches, blocks = w.blocks(), row_blocks = (M + 15) / 16, padded = row_blocks * 16;
+  const int first = (int)((long)stretches * blockIdx.y / gridDim.y), end = (int)((long)stretches * (blockIdx.y + 1) / gridDim.y);
+  const uint8_t* ap[XB];
+  const uint8_t* wp[YB];
+  const float* ws[YB];
+  const uint32_t* xp[XB];
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    const int block = min((tile_m * 2 + wm) * XB + x, row_blocks - 1);
+    ap[x] = a + (size_t)block * stretches * F8_BLOCK + lane * 16;
+    xp[x] = exponents + block * 16 + lane % 16;
+  }
+#pragma unroll
+  for (int y = 0; y < YB; ++y) {
+    const int block = min((tile_n * 2 + wn) * HALF + y % HALF, blocks - 1), matrix = y / HALF;
+    wp[y] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    ws[y] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+  }
+  f8_f32x4_t acc[XB][YB];
+#pragma unroll
+  for (int x = 0; x < XB; ++x)
+#pragma unroll
+    for (int y = 0; y < YB; ++y) acc[x][y] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f8_walk<FULL, XB, YB, F8_BLOCK, 1024>(ap, xp, padded, wp, ws, first, end, acc);
+  const int N = w.rows;
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    const int row = ((tile_m * 2 + wm) * XB + x) * 16 + lane % 16;
+    if (row >= M) continue;
+#pragma unroll
+    for (int y = 0; y < (PARTS ? YB : HALF); ++y) {
+      const int n = ((tile_n * 2 + wn) * HALF + y % HALF) * 16 + 4 * (lane / 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= N) break;
+        if constexpr (PARTS) {
+          const int width = GATED ? 2 * N : N;
+          reinterpret_cast<float*>(c)[((size_t)blockIdx.y * M + row) * width + (y / HALF) * N + n + e] = acc[x][y][e];
+        } else {
+          TC* at = c + (size_t)row * ldc + n + e;
+          float value = GATED ? gate_mul(acc[x][y][e], acc[x][y + (GATED ? HALF : 0)][e], form) : acc[x][y][e];
+          if (accumulate) value += to_f32(*at);
+          *at = from_f32<TC>(value);
+        }
+      }
+    }
+  }
+}
+
+// The parts' sums in their order.  grid (ceil(N / 256), M).
+template <typename TC, bool GATED>
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ sums, TC* __restrict__ c, int parts, int N, int ldc, int accumulate,
+                                                     GateForm form) {
+  const int n = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y, M = gridDim.y, width = GATED ? 2 * N : N;
+  if (n >= N) return;
+  float sum[GATED ? 2 : 1];
+#pragma unroll
+  for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+    sum[g] = 0.f;
+    for (int p = 0; p < parts; ++p) sum[g] += sums[((size_t)p * M + row) * width + g * N + n];
+  }
+  TC* at = c + (size_t)row * ldc + n;
+  float value = GATED ? gate_mul(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
+  if (accumulate) value += to_f32(*at);
+  *at = from_f32<TC>(value);
+}
+
+// ---- which kernel ----------------------------------------------------------------------------------------------
+constexpr int FEW_ROWS = 32, MOST_PARTS = 16;
+
+int parts_of(int M, int N, int K, bool gated) {
+  const long tiles = (long)((M + 63) / 64) * ((N + (gated ? 63 : 127)) / (gated ? 64 : 128));
+  const int stretches = (K + F8_K - 1) / F8_K;
+  const long units = 2L * bh_compute_units();
+  const int wanted = (int)(tiles >= units ? 1 : (units + tiles - 1) / tiles);
+  const int most = stretches / 4 < MOST_PARTS ? stretches / 4 : MOST_PARTS;
+  return wanted < most ? wanted : most > 1 ? most : 1;
+}
+
+template <typename T, typename TC, bool GATED, bool FULL>
+void launch_few(const void* x, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
+  const bool whole = K % 8 == 0 && (uintptr_t)x % 16 == 0;
+  const dim3 grid(w.blocks());
+#define BH_F8_FEW(MB, WHOLE) few_kernel<T, TC, MB, 1, GATED, FULL, WHOLE><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)x, w, c, M, K, ldc, accumulate, form)
+  if (M <= 16) {
+    if (whole) BH_F8_FEW(1, true);
+    else BH_F8_FEW(1, false);
+  } else if (whole) BH_F8_FEW(2, true);
+  else BH_F8_FEW(2, false);
+#undef BH_F8_FEW
+}
+
+template <typename TC, bool GATED, bool FULL>
+void launch_tiles(const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, float* sums, int parts, int M, int ldc, int accumulate,
+                  GateForm form, hipStream_t stream) {
+  const dim3 grid((unsigned)(((long)(M + 63) / 64) * ((w.rows + (GATED ? 63 : 127)) / (GATED ? 64 : 128))), parts);
+  if (parts == 1) {
+    tiles_kernel<TC, GATED, FULL, false><<<grid, 256, 0, stream>>>(a, exponents, w, c, M, ldc, accumulate, form);
+    return;
+  }
+  tiles_kernel<float, GATED, FULL, true><<<grid, 256, 0, stream>>>(a, exponents, w, sums, M, ldc, 0, form);
+  finish_kernel<TC, GATED><<<dim3((w.rows + 255) / 256, M), 256, 0, stream>>>(sums, c, parts, w.rows, ldc, accumulate, form);
+}
+
+int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int M, int N, int K, int ldc, int gate) {
+  BH_REQUIRE(M > 0 && N > 0 && K > 0, "gemm_float8: sizes must be positive, got %d x %d x %d", M, N, K);
+  BH_REQUIRE(K <= (1 << 24) && N <= (1 << 24) && ldc >= N, "gemm_float8: a product of %d outputs of %d inputs, rows %d apart", N, K, ldc);
+  BH_REQUIRE((uintptr_t)w % 16 == 0 && scales != nullptr && c != nullptr, "gemm_float8: the weight must be 16-byte aligned");
+  BH_REQUIRE(c_dtype == BH_F32 || c_dtype == BH_BF16, "gemm_float8: unknown output dtype %d", c_dtype);
+  BH_REQUIRE(gate == 0 || gate == BH_GATE_SILU || gate == BH_GATE_GELU_TANH, "gemm_float8: unknown gate %d", gate);
+  return 0;
+}
+
+}  // namespace
+
+// Whether a product of M rows takes them as they are (`few`); otherwise they are brought into 8 bits first.
+extern "C" int bh_gemm_float8_takes_rows(int M) { return M <= FEW_ROWS; }
+// Bytes of scratch memory of a product from rows in 8 bits.
+extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const int parts = parts_of(M, N, K, gated != 0);
+  return parts > 1 ? (long)parts * M * N * (gated ? 2 : 1) * 4 : 0;
+}
+
+#define BH_F8_BY_TYPES(RUN)                                                                                        \
+  do {                                                                                                             \
+    if (gate) {                                                                                                    \
+      if (c_dtype == BH_F32) { if (full) RUN(float, true, true); else RUN(float, true, false); }                   \
+      else { if (full) RUN(bf16_t, true, true); else RUN(bf16_t, true, false); }                                   \
+    } else if (c_dtype == BH_F32) { if (full) RUN(float, false, true); else RUN(float, false, false); }            \
+    else { if (full) RUN(bf16_t, false, true); else RUN(bf16_t, false, false); }                                   \
+  } while (0)
+
+// N: the outputs; of a gated product `w` holds two matrices of N rows, gate then up.  ldc: elements from a row of C to the next.
+extern "C" int bh_gemm_float8_few(const void* x, int dtype, const void* w, const void* scales, void* c, int c_dtype, int accumulate, int M, int N,
+                                  int K, int ldc, int gate, int full, hipStream_t stream) {
+  if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
+  BH_REQUIRE(M <= FEW_ROWS, "gemm_float8_few: up to %d rows, got %d", FEW_ROWS, M);
+  BH_REQUIRE(dtype == BH_F32 || dtype == BH_BF16, "gemm_float8_few: unknown dtype %d", dtype);
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+  const GateForm form = bh_gate_form(gate);
+#define BH_F8_RUN(TC, GATED, FULL)                                                                                     \
+  do {                                                                                                                 \
+    if (dtype == BH_F32) launch_few<float, TC, GATED, FULL>(x, weight, (TC*)c, M, K, ldc, accumulate, form, stream);   \
+    else launch_few<bf16_t, TC, GATED, FULL>(x, weight, (TC*)c, M, K, ldc, accumulate, form, stream);                  \
+  } while (0)
+  BH_F8_BY_TYPES(BH_F8_RUN);
+#undef BH_F8_RUN
+  return bh_check_launch("gemm_float8_few");
+}
+
+extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* w, const void* scales, void* c, int c_dtype, int accumulate, int M,
+                              int N, int K, int ldc, int gate, int full, void* scratch, hipStream_t stream) {
+  if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
+  BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
+  const int parts = parts_of(M, N, K, gate != 0);
+  BH_REQUIRE(parts == 1 || scratch != nullptr, "gemm_float8: a product in %d parts needs scratch memory", parts);
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+  const GateForm form = bh_gate_form(gate);
+#define BH_F8_RUN(TC, GATED, FULL) \
+  launch_tiles<TC, GATED, FULL>((const uint8_t*)a, (const uint32_t*)exponents, weight, (TC*)c, (float*)scratch, parts, M, ldc, accumulate, form, stream)
+  BH_F8_BY_TYPES(BH_F8_RUN);
+#undef BH_F8_RUN
+  return bh_check_launch("gemm_float8");
+}

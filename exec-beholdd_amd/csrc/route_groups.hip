@@ -1,0 +1,163 @@
+// The router of a mixture of experts whose rows use experts of a few groups only (HipKernels.route_in_groups).
+//   score[e]  = 1 / (1 + exp(-z[e]))  or  exp(z[e] - max z) / sum exp(z - max z)          z: a row's E logits
+//   by[e]     = score[e] + correction[e]                                                  what is chosen by
+//   merit[g]  = the largest of by in group g, or the sum of its two largest; groups are runs of E / groups neighbours
+//   chosen    = the `top` largest of by in the `keep` groups of largest merit, largest first; ties go to the lower index
+//   weights   = score of the chosen, divided by their sum where asked for, times `factor`
+// A row is a wave's.  Choices are whole numbers that a rounding would change, and scores of two experts differ by less than 32 bits tell
+// apart in one row of 30,000 (256 experts): scores, merits and sums are in 64 bits, whose exponentials are a small part of the time.
+// A score that is not a number counts as the lowest, so that the indices are always `top` different experts of open groups.
+#include "common.h"
+
+#define RG_MAX_TOP 32
+#define RG_MAX_GROUPS 64
+#define RG_WAVES 4
+
+namespace {
+
+struct Two {
+  double first, second;
+};
+__device__ inline Two merged(Two a, Two b) {
+  const bool mine = a.first >= b.first;
+  return {mine ? a.first : b.first, mine ? fmax(a.second, b.first) : fmax(b.second, a.first)};
+}
+
+__device__ inline double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = BH_WAVE / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, BH_WAVE);
+  return v;
+}
+
+// PER: experts a lane holds (lane, lane + 64, ...).  LDS: by of the wave's row, E doubles a wave.
+template <int PER>
+__global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float* __restrict__ logits, int stride, const float* __restrict__ correction,
+                                                                    int32_t* __restrict__ chosen, float* __restrict__ weights, int n_rows, int E, int top,
+                                                                    int groups, int keep, int softmax, int top_two, int renorm, float factor) {
+  extern __shared__ double by_of[];
+  const int lane = threadIdx.x % BH_WAVE, wave = threadIdx.x / BH_WAVE, row = blockIdx.x * RG_WAVES + wave;
+  if (row >= n_rows) return;      // nothing below meets other waves
+  const float* z = logits + (size_t)row * stride;
+  double* by_row = by_of + (size_t)wave * E;
+  const double none = -__builtin_inf();
+  double score[PER], by[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + i * BH_WAVE;
+    score[i] = e < E ? (double)z[e] : none;
+  }
+  if (softmax) {
+    double most = none, total = 0.;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) most = fmax(most, score[i]);
+#pragma unroll
+    for (int off = BH_WAVE / 2; off > 0; off >>= 1) most = fmax(most, __shfl_xor(most, off, BH_WAVE));
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      score[i] = lane + i * BH_WAVE < E ? exp(score[i] - most) : 0.;
+      total += score[i];
+    }
+    total = wave_sum_f64(total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) score[i] /= total;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) score[i] = 1. / (1. + exp(-score[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + i * BH_WAVE;
+    by[i] = e < E ? score[i] + (correction ? (double)correction[e] : 0.) : none;
+    if (!(by[i] == by[i])) by[i] = none;
+  }
+  unsigned taken = 0;      // bit i: this lane's expert lane + 64 i may not be chosen (any more)
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (lane + i * BH_WAVE >= E) taken |= 1u << i;
+  if (keep < groups) {
+    const int each = E / groups;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + i * BH_WAVE < E) by_row[lane + i * BH_WAVE] = by[i];
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int room = 1;      // groups rounded up to a power of two: 64 / room lanes look through a group
+    while (room < groups) room *= 2;
+    const int lanes = BH_WAVE / room, group = lane / lanes;
+    Two best = {none, none};
+    if (group < groups)
+      for (int i = lane % lanes; i < each; i += lanes) best = merged(best, Two{by_row[group * each + i], none});
+    for (int off = lanes / 2; off > 0; off >>= 1) best = merged(best, Two{__shfl_xor(best.first, off, BH_WAVE), __shfl_xor(best.second, off, BH_WAVE)});
+    const double merit = top_two && each > 1 ? best.first + best.second : best.first;
+    int better = 0;      // groups ahead of this lane's
+    for (int g = 0; g < groups; ++g) {
+      const double other = __shfl(merit, g * lanes, BH_WAVE);
+      better += other > merit || (other == merit && g < group) ? 1 : 0;
+    }
+    const unsigned long long open = __ballot(group < groups && better < keep);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane + i * BH_WAVE;
+      if (e < E && !((open >> (e / each * lanes)) & 1ull)) taken |= 1u << i;
+    }
+  }
+  double sum = 0., mine = 0.;      // lane j keeps the j-th choice
+  int mine_index = 0;
+  for (int j = 0; j < top; ++j) {
+    double best = none, best_score = 0.;
+    int best_e = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (!((taken >> i) & 1u) && (by[i] > best || best_e == 0x7fffffff)) {
+        best = by[i];
+        best_score = score[i];
+        best_e = lane + i * BH_WAVE;
+      }
+#pragma unroll
+    for (int off = BH_WAVE / 2; off > 0; off >>= 1) {
+      const double other = __shfl_xor(best, off, BH_WAVE), other_score = __shfl_xor(best_score, off, BH_WAVE);
+      const int other_e = __shfl_xor(best_e, off, BH_WAVE);
+      if (other_e != 0x7fffffff && (best_e == 0x7fffffff || other > best || (other == best && other_e < best_e))) {
+        best = other;
+        best_score = other_score;
+        best_e = other_e;
+      }
+    }
+    if (best_e % BH_WAVE == lane) taken |= 1u << (best_e / BH_WAVE);
+    sum += best_score;
+    if (lane == j) {
+      mine = best_score;
+      mine_index = best_e;
+    }
+  }
+  if (lane < top) {
+    if (renorm) mine = sum == 0. ? 0. : mine / sum;
+    chosen[(size_t)row * top + lane] = mine_index;
+    weights[(size_t)row * top + lane] = (float)(mine * (double)factor);
+  }
+}
+
+}  // namespace
+
+// logits [n_rows][stride]: a row's E logits are its first.
+extern "C" int bh_route_in_groups(const float* logits, int stride, const float* correction, int32_t* chosen, float* weights, int n_rows, int E, int top,
+                                  int groups, int keep, int softmax, int top_two, int renorm, float factor, hipStream_t stream) {
+  BH_REQUIRE(n_rows > 0 && E > 0 && E <= 1024, "route_in_groups: 1 to 1024 experts, got %d", E);
+  BH_REQUIRE(stride >= E, "route_in_groups: %d logits do not lie in a row of %d", E, stride);
+  BH_REQUIRE(groups >= 1 && groups <= RG_MAX_GROUPS && E % groups == 0, "route_in_groups: %d experts do not make 1 to %d equal groups of which there are %d",
+             E, RG_MAX_GROUPS, groups);
+  BH_REQUIRE(keep >= 1 && keep <= groups, "route_in_groups: a row uses 1 to %d groups, got %d", groups, keep);
+  BH_REQUIRE(top >= 1 && top <= RG_MAX_TOP && (long)top <= (long)keep * (E / groups), "route_in_groups: 1 to min(%d, %ld) experts a row, got %d",
+             RG_MAX_TOP, (long)keep * (E / groups), top);
+  const dim3 grid((n_rows + RG_WAVES - 1) / RG_WAVES);
+  const size_t lds = keep < groups ? (size_t)RG_WAVES * E * sizeof(double) : 0;
+#define BH_ROUTE(PER)                                                                                                                         \
+  route_groups_kernel<PER><<<grid, RG_WAVES * 64, lds, stream>>>(logits, stride, correction, chosen, weights, n_rows, E, top, groups, keep, \
+                                                                softmax, top_two, renorm, factor)
+  if (E <= BH_WAVE) BH_ROUTE(1);
+  else if (E <= 2 * BH_WAVE) BH_ROUTE(2);
+  else if (E <= 4 * BH_WAVE) BH_ROUTE(4);
+  else BH_ROUTE(16);
+#undef BH_ROUTE
+  return bh_check_launch("route_in_groups");
+}

@@ -108,6 +108,50 @@ class BothRows:
         return 2
 
 
+class Float8Weight:
+    """One or more weight matrices of equal size in 8-bit floating point (e4m3), one below the other, with a float32 scale for each
+    block of 128 x 128 of each: `HipKernels.pack_float8` makes it, `gemm`, `gemm_swiglu` and `experts_float8` take it.  `data` holds the
+    values in blocks of 16 rows x 128 columns in matrix-core operand order (csrc/float8.h), `scales` is [matrices, blocks of rows,
+    blocks of columns].  `shape` is that of the stacked matrices."""
+
+    BLOCK = 128
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, matrices: int, rows: int, cols: int):
+        self.data, self.scales, self.matrices, self.rows = data, scales, int(matrices), int(rows)
+        self.shape, self.dtype, self.device = (self.matrices * self.rows, int(cols)), torch.float8_e4m3fn, data.device
+
+    def dim(self):
+        return 2
+
+    @staticmethod
+    def data_bytes(matrices: int, rows: int, cols: int) -> int:
+        return matrices * (-(-rows // 16) * 16) * (-(-cols // 128) * 128)
+
+    @staticmethod
+    def scale_shape(matrices: int, rows: int, cols: int) -> tuple:
+        return (matrices, -(-rows // 128), -(-cols // 128))
+
+
+class Float8Rows:
+    """Activation rows in 8-bit floating point with a power of two for each stretch of 128 columns of a row: what products with a
+    `Float8Weight` read where the rows are many.  `HipKernels.to_float8` makes it.  `data` holds whole stretches, in blocks of 16 rows x
+    128 columns in matrix-core operand order, or row after row (`in_rows`); `exponents` int32 [ceil(width / 512), rows padded to 16] holds
+    four exponents a word (csrc/float8.h).  `shape` is that of the matrix."""
+
+    def __init__(self, data: torch.Tensor, exponents: torch.Tensor, rows: int, width: int, in_rows: bool = False):
+        self.data, self.exponents, self.in_rows = data, exponents, bool(in_rows)
+        self.shape, self.dtype, self.device = (int(rows), int(width)), torch.float8_e4m3fn, data.device
+
+    def dim(self):
+        return 2
+
+    @staticmethod
+    def bytes_of(rows: int, width: int) -> tuple:
+        """(bytes of the values, bytes of the exponents)."""
+        padded = -(-rows // 16) * 16
+        return padded * (-(-width // 128) * 128), 4 * padded * -(-width // 512)
+
+
 def _block_rows(x) -> int:
     """In blocks of how many rows a matrix lies (0: row after row)."""
     return x.block_rows if isinstance(x, BlockedRows) else 0
@@ -255,11 +299,21 @@ class KernelSizes:
             "bh_slice_rmsnorm": [p, i, i, i, p, f, p, i, i, i, p],
             "bh_weighted_sum": [p, p, f, p, f, ctypes.c_long, p],
             "bh_experts_combine": [p, p, p, p, p, i, p, i, i, i, i, i, p],
+            "bh_float8_rows": [p, i, p, p, i, i, i, i, p],
+            "bh_gemm_float8_takes_rows": [i],
+            "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
+            "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
+            "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
+            "bh_experts_float8_few": [i, i],
+            "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
+            "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
+            "bh_experts_float8_sum": [p, p, p, p, i, p, i, i, i, i, i, i, p],
         }
         for name, argtypes in table.items():
             function = getattr(lib, name)
             function.argtypes = argtypes
             function.restype = i
+        lib.bh_gemm_float8_scratch.argtypes, lib.bh_gemm_float8_scratch.restype = [i, i, i, i], ctypes.c_long
         lib.bh_gemm_bf16_scratch.argtypes = [i, i, i, i, i]
         lib.bh_gemm_bf16_scratch.restype = ctypes.c_long
         for query, count in ((lib.bh_lightning_products_scratch, 10), (lib.bh_ssm_products_scratch, 8), (lib.bh_lightning_products_most, 6),
@@ -624,9 +678,11 @@ class HipKernels(KernelSizes):
         reader = getattr(then_norm, "reader", None)
         return (reader.outputs, reader.swiglu, getattr(reader, "packed", True)) if reader is not None else ()
 
-    def gemm(self, a, w, out, accumulate=False, then_norm=None):
+    def gemm(self, a, w, out, accumulate=False, then_norm=None, full_sums=None):
         """out[M, N] (+)= a[M, K] @ w[N, K]^T with float32 accumulation; `w` may be a PackedWeight and
-        `a` the NormedRows an earlier product prepared.  With `then_norm` (an object with `weight` [N] and
+        `a` the NormedRows an earlier product prepared.  With a `Float8Weight` the rows go into the product in 8 bits too (`to_float8`);
+        `full_sums` says whether its sums are those of float32 (if not said: where `out` is float32) or the 8-bit matrix cores', which
+        drop what lies 2^14 below the largest of 8 neighbouring products, at up to twice the rate.  With `then_norm` (an object with `weight` [N] and
         `eps`: an RMSNorm over the rows of `out` as they are after this product) the product may prepare that norm's
         output on its way and return it, as NormedRows or, where it finishes the norm itself, as the bfloat16
         matrix the norm would have given; it returns None when it does neither (then run the norm as usual)."""
@@ -636,6 +692,9 @@ class HipKernels(KernelSizes):
         n = w.shape[0]
         if w.shape[1] != k or tuple(out.shape) != (m, n):
             raise KernelError(f"gemm: shapes a {tuple(a.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)} do not fit")
+        if isinstance(w, Float8Weight):
+            self._gemm_float8(a, w, out, accumulate, 0, full_sums)
+            return None
         if isinstance(a, NormedRows) and a.ss is None and not accumulate and self._normed_f32(a, w, out, n, 0):
             return None
         if isinstance(a, NormedRows) and (a.ss is None or not self._takes_norm(a, w, n, 0)):
@@ -779,13 +838,19 @@ class HipKernels(KernelSizes):
         self.rmsnorm(prepared.source, prepared.weight, prepared.eps, out)
         return out
 
-    def gemm_swiglu(self, a, w, out, gate="silu"):
+    def gemm_swiglu(self, a, w, out, gate="silu", full_sums=None):
         """out[M, F] = silu(a @ w[:F]^T) * (a @ w[F:]^T) for w [2F, K] = gate rows, then up rows; `a` may
-        be NormedRows.  `gate`: "silu", or "gelu_tanh" for GELU's tanh form in its place."""
+        be NormedRows.  `gate`: "silu", or "gelu_tanh" for GELU's tanh form in its place.  A `Float8Weight` of two matrices goes as in
+        `gemm`, with an output of either type."""
         if a.dim() != 2 or w.dim() != 2 or out.dim() != 2:
             raise KernelError("gemm_swiglu: operands must be matrices")
         m, k = a.shape
         width = out.shape[1]
+        if isinstance(w, Float8Weight):
+            if w.matrices != 2 or tuple(w.shape) != (2 * width, k) or out.shape[0] != m:
+                raise KernelError(f"gemm_swiglu: shapes a {tuple(a.shape)}, w {w.matrices} matrices {tuple(w.shape)}, out {tuple(out.shape)} do not fit")
+            self._gemm_float8(a, w, out, False, self.GATES[gate], full_sums)
+            return
         if tuple(w.shape) != (2 * width, k) or out.shape[0] != m or out.dtype != a.dtype:
             raise KernelError(f"gemm_swiglu: shapes a {tuple(a.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)} "
                               "do not fit")
@@ -809,6 +874,169 @@ class HipKernels(KernelSizes):
         both = torch.empty((m, 2 * width), dtype=a.dtype, device=self.device)
         self.gemm(a, w, both)
         self.swiglu(both, out, gate)
+
+    # ---- weights and rows in 8 bits ----
+    def pack_float8(self, w, scales=None, matrices=1) -> Float8Weight:
+        """`w` [matrices * rows, K] as a `Float8Weight`.  A float32 or bfloat16 matrix is quantised: a block's scale is its largest
+        magnitude / 448 (1 for a block of zeros), a value the nearest e4m3 of value / scale.  A float8_e4m3fn matrix is taken as it is, with
+        its `scales` float32 [matrices, ceil(rows / 128), ceil(K / 128)] (or without the first axis).  Every value must be finite."""
+        if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.device != self.device or w.numel() == 0:
+            raise KernelError(f"pack_float8: a matrix on {self.device}, got {getattr(w, 'shape', type(w))} on {getattr(w, 'device', None)}")
+        if scales is not None:
+            if w.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32 or scales.device != self.device or scales.dim() not in (2, 3):
+                raise KernelError("pack_float8: scales (float32, [matrices, blocks of rows, blocks of columns]) go with float8_e4m3fn values")
+            scales = scales if scales.dim() == 3 else scales[None]
+            matrices = scales.shape[0]
+        elif w.dtype not in _CODES:
+            raise KernelError(f"pack_float8: dtype {w.dtype} is not float32, bfloat16 or float8_e4m3fn with scales")
+        matrices = int(matrices)
+        if matrices < 1 or w.shape[0] % matrices:
+            raise KernelError(f"pack_float8: {w.shape[0]} rows are not those of {matrices} equal matrices")
+        rows, cols = w.shape[0] // matrices, w.shape[1]
+        n_blocks, k_blocks = -(-rows // 128), -(-cols // 128)
+        if scales is not None and tuple(scales.shape) != Float8Weight.scale_shape(matrices, rows, cols):
+            raise KernelError(f"pack_float8: scales {tuple(scales.shape)} for {matrices} matrices of {rows} x {cols}")
+        padded = -(-rows // 16) * 16
+        data = torch.empty((matrices, padded * k_blocks * 128), dtype=torch.uint8, device=self.device)
+        kept = torch.empty((matrices, n_blocks, k_blocks), dtype=torch.float32, device=self.device)
+        sound = torch.ones((), dtype=torch.bool, device=self.device)
+        for i in range(matrices):
+            one = w[i * rows:(i + 1) * rows]
+            if scales is None:
+                whole = torch.zeros((n_blocks * 128, k_blocks * 128), dtype=torch.float32, device=self.device)
+                whole[:rows, :cols] = one
+                blocks = whole.view(n_blocks, 128, k_blocks, 128)
+                largest = blocks.abs().amax(dim=(1, 3))
+                kept[i] = torch.where(largest > 0, largest / torch.full_like(largest, 448.0), torch.ones_like(largest)).clamp(min=2.0 ** -126)
+                values = (blocks / kept[i][:, None, :, None]).view(whole.shape)[:padded].to(torch.float8_e4m3fn).view(torch.uint8)
+            else:
+                kept[i] = scales[i]
+                values = torch.zeros((padded, k_blocks * 128), dtype=torch.uint8, device=self.device)
+                values[:rows, :cols] = one.contiguous().view(torch.uint8)
+            sound &= torch.isfinite(kept[i]).all() & ~((values & 0x7f) == 0x7f).any()
+            # [block of 16 rows][block of 128 k][half h of 64][lane group q][row][16]
+            data[i] = values.view(padded // 16, 16, k_blocks, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).reshape(-1)
+        if not bool(sound):
+            raise KernelError("pack_float8: the matrix or its scales hold an infinity or a NaN")
+        return Float8Weight(data.view(-1), kept, matrices, rows, cols)
+
+    def unpack_float8(self, w) -> torch.Tensor:
+        """The float32 matrix that a `Float8Weight` stands for."""
+        (total, cols), k_blocks, padded = w.shape, -(-w.shape[1] // 128), -(-w.rows // 16) * 16
+        values = w.data.view(w.matrices, padded // 16, k_blocks, 2, 4, 16, 16).permute(0, 1, 5, 2, 3, 4, 6).reshape(w.matrices, padded, k_blocks * 128)
+        spread = w.scales.repeat_interleave(128, dim=1)[:, :w.rows].repeat_interleave(128, dim=2)[:, :, :cols]
+        return (values[:, :w.rows, :cols].contiguous().view(torch.float8_e4m3fn).to(torch.float32) * spread).reshape(total, cols)
+
+    def to_float8(self, x, gate=None, in_rows=False) -> Float8Rows:
+        """The rows `x` [n, K] (float32 or bfloat16) as `Float8Rows`: a stretch of 128 columns of a row has the scale 2^e with the least
+        e >= -126 for which no magnitude exceeds 448 * 2^e, a value is the nearest e4m3 of value / 2^e; a value that is not finite becomes NaN.
+        With `gate` ("silu" or "gelu_tanh") the rows are [gate | up] and what is quantised is gate's activation times up."""
+        if gate is not None and gate not in self.GATES:
+            raise KernelError(f"to_float8: a gate is one of {sorted(self.GATES)}, got {gate!r}")
+        if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] % (2 if gate else 1):
+            raise KernelError(f"to_float8: a matrix (of an even width with a gate), got {getattr(x, 'shape', type(x))}")
+        rows, width = x.shape[0], x.shape[1] // (2 if gate else 1)
+        data_bytes, exponent_bytes = Float8Rows.bytes_of(rows, width)
+        out = Float8Rows(torch.empty(data_bytes, dtype=torch.uint8, device=self.device),
+                         torch.empty((-(-width // 512), exponent_bytes // 4 // -(-width // 512)), dtype=torch.int32, device=self.device), rows, width, in_rows)
+        self._check(self.lib.bh_float8_rows(self._ptr(x, "rows"), _code(x, "rows"), out.data.data_ptr(), out.exponents.data_ptr(), rows, width,
+                                            int(out.in_rows), self.GATES[gate] if gate else 0, self._stream()))
+        return out
+
+    def from_float8(self, x) -> torch.Tensor:
+        """The float32 matrix that `Float8Rows` stand for."""
+        (rows, width), stretches, padded = x.shape, -(-x.shape[1] // 128), -(-x.shape[0] // 16) * 16
+        if x.in_rows:
+            values = x.data.view(padded, stretches * 128)
+        else:
+            values = x.data.view(padded // 16, stretches, 2, 4, 16, 16).permute(0, 4, 1, 2, 3, 5).reshape(padded, stretches * 128)
+        exponents = x.exponents.view(torch.uint8).view(-1, padded, 4).permute(1, 0, 2).reshape(padded, -1)[:rows, :stretches]
+        scale = torch.ldexp(torch.ones((), dtype=torch.float32, device=self.device), exponents.to(torch.int32) - 127)
+        return values[:rows, :width].contiguous().view(torch.float8_e4m3fn).to(torch.float32) * scale.repeat_interleave(128, dim=1)[:, :width]
+
+    def _plain_rows(self, a):
+        """Activations in any of the library's forms as a plain matrix."""
+        if isinstance(a, NormedRows):
+            out = torch.empty(tuple(a.shape), dtype=a.dtype, device=self.device)
+            self.rmsnorm(a.source, a.weight, a.eps, out)
+            return out
+        return self._in_blocks_of(a, 0)
+
+    def _gemm_float8(self, a, w, out, accumulate, gate, full_sums):
+        """out (+)= a times a `Float8Weight`, plain (gate 0) or gated."""
+        (m, k), n, matrices = a.shape, w.rows, 1 if gate else w.matrices
+        full = out.dtype == torch.float32 if full_sums is None else bool(full_sums)
+        if isinstance(out, BlockedRows):
+            raise KernelError("gemm: a product with an 8-bit weight writes plain rows")
+        if isinstance(a, Float8Rows):
+            if a.in_rows:
+                raise KernelError("gemm: rows in 8 bits go into a product in blocks")
+        else:
+            a = self._plain_rows(a)
+            if not self.lib.bh_gemm_float8_takes_rows(m):
+                self._ptr(a, "gemm a", tuple(_CODES))
+                a = self.to_float8(a)
+        out_at, c_code, stream = self._ptr(out, "gemm out"), _code(out, "gemm out"), self._stream()
+        for i in range(matrices):
+            data = w.data.data_ptr() + i * Float8Weight.data_bytes(1, n, k)
+            scales, at = w.scales.data_ptr() + i * w.scales[0].numel() * 4, out_at + i * n * out.element_size()
+            if not isinstance(a, Float8Rows):
+                self._check(self.lib.bh_gemm_float8_few(self._ptr(a, "gemm a"), _code(a, "gemm a"), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
+                                                        out.shape[1], gate, int(full), stream))
+                continue
+            scratch_bytes = int(self.lib.bh_gemm_float8_scratch(m, n, k, int(gate != 0)))
+            scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=self.device) if scratch_bytes else None
+            self._check(self.lib.bh_gemm_float8(a.data.data_ptr(), a.exponents.data_ptr(), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
+                                                out.shape[1], gate, int(full), scratch.data_ptr() if scratch is not None else None, stream))
+
+    def experts_float8(self, x, chosen, weights, w_up, w_down, out, limit=float("inf"), alpha=1.0, shift=0.0, weigh_input=False, fresh=False, through=None,
+                       full_sums=None):
+        """out[r] += sum_j weights[r, j] * Wd_e act(Wg_e x[r], Wu_e x[r]), e = chosen[r, j], j in order (`fresh`: written, not added), with
+        act(g, u) = g' sigmoid(alpha g') (u' + shift), g' = min(g, limit), u' = clamp(u, -limit, limit).  x [n, K] float32 or bfloat16,
+        chosen int32 [n, top], weights float32 [n, top]; `w_up` a `Float8Weight` of 2 E matrices [ff, K] (gate and up of each expert in turn),
+        `w_down` one of E matrices [D, ff], out [n, D] float32 or bfloat16.  `weigh_input`: a pair's weight multiplies the expert's input in
+        place of its output.  A pair whose expert is none of the E counts nothing; with `through` [n, D] (of x's type) one that is numbered
+        E or higher gives through[r].  x and the activations go into the products in 8 bits (`to_float8`); `full_sums` as in `gemm`, but if it
+        is not said the gate and up sums are full: they are rounded to 8 bits, and each that falls on the other side of a border is a whole
+        step off (4,096 rows of 4,096, bfloat16 output: 2.6e-3 of it, 1.7e-3 with full sums, where its own rounding is 1.6e-3)."""
+        if not isinstance(w_up, Float8Weight) or not isinstance(w_down, Float8Weight) or x.dim() != 2 or chosen.dim() != 2:
+            raise KernelError("experts_float8: rows, choices [n, top] and two 8-bit weights")
+        (n, k), top, experts, ff, width = x.shape, chosen.shape[1], w_down.matrices, w_up.rows, w_down.rows
+        if (w_up.matrices != 2 * experts or w_up.shape[1] != k or w_down.shape[1] != ff or tuple(out.shape) != (n, width) or chosen.shape[0] != n
+                or (weights is not None and weights.shape != chosen.shape) or (weights is None and weigh_input)
+                or not self._goes_through(through, n, width, x.dtype)):
+            raise KernelError(f"experts_float8: shapes x {tuple(x.shape)}, chosen {tuple(chosen.shape)}, weights {w_up.matrices} x {w_up.rows} x {w_up.shape[1]} "
+                              f"and {experts} x {width} x {w_down.shape[1]}, out {tuple(out.shape)} do not fit")
+        if through is not None and weigh_input:
+            raise KernelError("experts_float8: inputs that are handed through are weighed on their way out")
+        full, full_up = out.dtype == torch.float32 if full_sums is None else bool(full_sums), full_sums is None or bool(full_sums)
+        lib, stream, pairs = self.lib, self._stream(), n * top
+        chosen_at, weights_at = self._ptr(chosen, "chosen", (torch.int32,)), self._ptr(weights, "route weights", (torch.float32,), True)
+        act = (float(limit), float(alpha), float(shift))
+        x_at, x_code, out_at, out_code = self._ptr(x, "experts x"), _code(x, "experts x"), self._ptr(out, "experts out"), _code(out, "experts out")
+        through_at = self._ptr(through, "experts input", None, True)
+        inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
+        y = torch.empty((pairs, width), dtype=torch.float32, device=self.device)
+        in_weights = weights_at if weigh_input else None
+        if lib.bh_experts_float8_few(pairs, experts):
+            self._check(lib.bh_experts_float8_rows(x_at, x_code, top, chosen_at, pairs, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(),
+                                                   ff, k, 1, *act, in_weights, int(full_up), stream))
+            self._check(lib.bh_experts_float8_rows(inner.data_ptr(), F32, 1, chosen_at, pairs, experts, w_down.data.data_ptr(), w_down.scales.data_ptr(),
+                                                   y.data_ptr(), width, ff, 0, *act, None, int(full), stream))
+        else:
+            lists = torch.empty((experts, pairs), dtype=torch.int32, device=self.device)      # a row may name an expert more than once
+            counts = torch.empty((experts,), dtype=torch.int32, device=self.device)
+            self._check(lib.bh_experts_group(chosen_at, pairs, lists.data_ptr(), pairs, counts.data_ptr(), experts, stream))
+            rows = self.to_float8(x, in_rows=True)
+            self._check(lib.bh_experts_float8_tiles(rows.data.data_ptr(), rows.exponents.data_ptr(), n, top, lists.data_ptr(), pairs, counts.data_ptr(), pairs,
+                                                    experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(), ff, k, 1, *act, in_weights,
+                                                    int(full_up), stream))
+            rows = self.to_float8(inner, in_rows=True)
+            self._check(lib.bh_experts_float8_tiles(rows.data.data_ptr(), rows.exponents.data_ptr(), pairs, 1, lists.data_ptr(), pairs, counts.data_ptr(), pairs,
+                                                    experts, w_down.data.data_ptr(), w_down.scales.data_ptr(), y.data_ptr(), width, ff, 0, *act, None,
+                                                    int(full), stream))
+        self._check(lib.bh_experts_float8_sum(y.data_ptr(), chosen_at, None if weigh_input else weights_at, through_at, x_code, out_at, out_code, n, experts, top,
+                                              width, int(bool(fresh)), stream))
 
     def qk_norm_rope_cache(self, qkv, q_out, q_weight, k_weight, eps, cos, sin, positions, row_seq,
                            k_pages, v_pages, page_table, n_heads, n_kv_heads, head_dim, write_kv, max_position):
@@ -1844,6 +2072,27 @@ class HipKernels(KernelSizes):
             self._ptr(logits, "router logits", (torch.float32,)), stride, self._ptr(bias, "router bias", (torch.float32,), True),
             self._ptr(correction, "router correction", (torch.float32,), True), self._ptr(chosen, "chosen", (torch.int32,)), self._ptr(weights, "route weights", (torch.float32,)), n_rows, experts, top,
             self.SCORINGS[scoring], self._stream()))
+
+    def route_in_groups(self, logits, correction, chosen, weights, scoring="sigmoid", groups=1, keep=None, group_score="top2", renorm=True, factor=1.0,
+                        experts=None):
+        """Routing in which a row uses experts of `keep` of the `groups` runs of E / groups neighbours only: score = the sigmoid of a logit
+        (`scoring` "sigmoid") or its share of the softmax over all E ("softmax"); by = score + `correction` (f32 [E] or None); a group counts as
+        its largest `by` ("max") or the sum of its two largest ("top2"); chosen[r] = the `top` largest `by` of the groups kept, largest first, ties
+        to the lower index; weights[r] = `factor` * their scores, divided by their sum with `renorm` (0 where that is 0).  Scores and choices
+        are made in 64 bits; a `by` that is not a number counts as the lowest.  logits f32 [n, >= E], chosen int32 [n, top], weights f32 [n, top];
+        `experts`: how many of a row's first columns are logits (all where it is not said)."""
+        if scoring not in ("sigmoid", "softmax") or group_score not in ("max", "top2"):
+            raise KernelError(f"route_in_groups: scores 'sigmoid' or 'softmax' and groups by 'max' or 'top2', got {scoring!r} and {group_score!r}")
+        if logits.dim() != 2 or chosen.dim() != 2:
+            raise KernelError("route_in_groups: logits [n, E] and choices [n, top]")
+        n_rows, stride = logits.shape
+        experts, top, groups = int(experts) if experts is not None else stride, chosen.shape[1], int(groups)
+        if chosen.shape != (n_rows, top) or weights.shape != (n_rows, top) or (correction is not None and correction.shape != (experts,)):
+            raise KernelError(f"route_in_groups: shapes logits {tuple(logits.shape)}, chosen {tuple(chosen.shape)}, weights {tuple(weights.shape)} do not fit")
+        self._check(self.lib.bh_route_in_groups(
+            self._ptr(logits, "router logits", (torch.float32,)), stride, self._ptr(correction, "router correction", (torch.float32,), True),
+            self._ptr(chosen, "chosen", (torch.int32,)), self._ptr(weights, "route weights", (torch.float32,)), n_rows, experts, top, groups,
+            groups if keep is None else int(keep), int(scoring == "softmax"), int(group_score == "top2"), int(bool(renorm)), float(factor), self._stream()))
 
     def experts_gate_up(self, h, chosen, w_gate_up, inner, limit, alpha, shift=1.0, in_weights=None):
         """inner[r * top + j] = act(Wg_e h[r], Wu_e h[r]) for e = chosen[r, j]; w_gate_up [E, 2 ff, K] (gate rows, then up rows).
