@@ -3,6 +3,7 @@
 //   tiles   any number of rows, from rows in 8 bits (float8_rows.hip), K in parts where the tiles alone leave compute units idle
 #include "float8_few.h"
 #include "float8_tiles.h"
+#include "gemm_float8_ring.h"
 
 namespace {
 
@@ -228,8 +229,8 @@ int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int 
 // Whether a product of M rows takes them as they are (`few`); otherwise they are brought into 8 bits first.
 extern "C" int bh_gemm_float8_takes_rows(int M) { return M <= FEW_ROWS; }
 // Bytes of scratch memory of a product from rows in 8 bits.
-extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full) {
+  if (M <= 0 || N <= 0 || K <= 0 || float8_ring_tile(M, N, K, gated != 0, full != 0) >= 0) return 0;
   const int parts = parts_of(M, N, K, gated != 0);
   return parts > 1 ? (long)parts * M * N * (gated ? 2 : 1) * 4 : 0;
 }
@@ -265,6 +266,10 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
                               int N, int K, int ldc, int gate, int full, void* scratch, hipStream_t stream) {
   if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
   BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
+  const int tile = float8_ring_tile(M, N, K, gate != 0, full != 0);
+  if (tile >= 0)
+    return float8_ring_launch(tile, (const uint8_t*)a, (const uint32_t*)exponents, {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K}, c,
+                              c_dtype, accumulate, M, ldc, gate != 0, full, bh_gate_form(gate), stream);
   const int parts = parts_of(M, N, K, gate != 0);
   BH_REQUIRE(parts == 1 || scratch != nullptr, "gemm_float8: a product in %d parts needs scratch memory", parts);
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};

@@ -313,7 +313,7 @@ class KernelSizes:
             function = getattr(lib, name)
             function.argtypes = argtypes
             function.restype = i
-        lib.bh_gemm_float8_scratch.argtypes, lib.bh_gemm_float8_scratch.restype = [i, i, i, i], ctypes.c_long
+        lib.bh_gemm_float8_scratch.argtypes, lib.bh_gemm_float8_scratch.restype = [i, i, i, i, i], ctypes.c_long
         lib.bh_gemm_bf16_scratch.argtypes = [i, i, i, i, i]
         lib.bh_gemm_bf16_scratch.restype = ctypes.c_long
         for query, count in ((lib.bh_lightning_products_scratch, 10), (lib.bh_ssm_products_scratch, 8), (lib.bh_lightning_products_most, 6),
@@ -984,7 +984,7 @@ class HipKernels(KernelSizes):
                 self._check(self.lib.bh_gemm_float8_few(self._ptr(a, "gemm a"), _code(a, "gemm a"), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
                                                         out.shape[1], gate, int(full), stream))
                 continue
-            scratch_bytes = int(self.lib.bh_gemm_float8_scratch(m, n, k, int(gate != 0)))
+            scratch_bytes = int(self.lib.bh_gemm_float8_scratch(m, n, k, int(gate != 0), int(full)))
             scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=self.device) if scratch_bytes else None
             self._check(self.lib.bh_gemm_float8(a.data.data_ptr(), a.exponents.data_ptr(), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
                                                 out.shape[1], gate, int(full), scratch.data_ptr() if scratch is not None else None, stream))
