@@ -5,9 +5,9 @@
 // A pair's weight may multiply the expert's input instead (its gate and up sums).  A pair whose expert is none of the E gives nothing, or,
 // with `through`, one numbered E or higher hands the row's input on.  Nothing here depends on the routing on the host.
 //   few    an expert's pairs 16 at a time, quantised by the waves that multiply them (gemm_float8.hip's product of few rows)
-//   tiles  tiles of 64 pairs of an expert from rows in 8 bits, found from the experts' counts by every workgroup itself
+//   tiles  tiles of 64 or 128 pairs of an expert from rows in 8 bits, found from the experts' counts by every workgroup itself
 #include "float8_few.h"
-#include "float8_tiles.h"
+#include "float8_ring.h"
 
 namespace {
 
@@ -123,15 +123,30 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------
-// a: rows in 8 bits, row after row; the input of pair p is row p / in_div.
-template <bool GATED, bool FULL>
-__global__ __launch_bounds__(256) void experts_tiles8_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded, int in_div,
-                                                             const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
-                                                             F8Weight w, float* __restrict__ out, ExpertGate gate, const float* __restrict__ in_weights) {
-  constexpr int XB = 2, YB = 4, ROWS = 64, OUTS = GATED ? 64 : 128, HALF = GATED ? YB / 2 : YB;
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 2, wn = wave % 2;
-  const int n_tiles = (w.rows + OUTS - 1) / OUTS, stretches = w.stretches, blocks = w.blocks();
-  // the expert and the tile of pairs: a wave adds up 64 experts' tiles at a time; every wave of the workgroup finds the same
+// A workgroup of 2 x 4 waves owns 32 XB pairs of one expert and 256 of its weight rows (gated: gate and up rows of the same 128 outputs), on
+// the ring of float8_ring.h with rows picked through the expert's list.  The gated form's 128 outputs are a stretch of the next product's
+// k: they are brought into 8 bits here, a pair's largest found between the four waves that hold its row.
+// a: rows in 8 bits, row after row; the input of pair p is row p / in_div.  out: float32 [pairs][N]; gated: rows in 8 bits, row after row,
+// and their exponents, `out_padded` words a row of them.
+template <bool GATED, bool FULL, int XB>
+__global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded, int in_div,
+                                                              const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
+                                                              F8Weight w, void* __restrict__ out, uint8_t* __restrict__ out_exponents, int out_padded,
+                                                              ExpertGate gate, const float* __restrict__ in_weights) {
+  using Ring = F8Ring<FULL, XB, 4, 2, 4, 3, GATED ? 2 : 1>;
+  constexpr int YB = Ring::YB, HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS, WN = Ring::WN;
+  __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[Ring::R * Ring::PIECES * 64];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
+  const int N = w.rows, n_tiles = (N + OUTS - 1) / OUTS, steps = w.stretches, blocks = w.blocks();
+  // Tiles of pairs of all experts: a wave adds up 64 experts at a time; every wave of the workgroup finds the same.  Workgroups go to the
+  // eight XCDs in turn: every XCD takes a run of (expert, weight tile, tile of pairs) in this order.
+  int total = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) total += e0 + lane < E ? (counts[e0 + lane] + ROWS - 1) / ROWS : 0;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, BH_WAVE);
+  total *= n_tiles;
+  const int each = (total + 7) / 8, turn = blockIdx.x / 8, id = (blockIdx.x % 8) * each + turn;
+  if (turn >= each || id >= total) return;      // the whole workgroup
   int expert = -1, before = 0, count = 0, at = 0;
   for (int e0 = 0; e0 < E && expert < 0; e0 += 64) {
     const int own = e0 + lane < E ? counts[e0 + lane] : 0, tiles = (own + ROWS - 1) / ROWS * n_tiles;
@@ -141,80 +156,137 @@ __global__ __launch_bounds__(256) void experts_tiles8_kernel(const uint8_t* __re
       const int lower = __shfl_up(upto, off, BH_WAVE);
       if (lane >= off) upto += lower;
     }
-    const unsigned long long behind = __ballot(before + upto > (int)blockIdx.x);
+    const unsigned long long behind = __ballot(before + upto > id);
     if (behind) {
       const int l = __ffsll(behind) - 1;
       expert = e0 + l;
       count = __shfl(own, l, BH_WAVE);
-      at = (int)blockIdx.x - before - (__shfl(upto, l, BH_WAVE) - __shfl(tiles, l, BH_WAVE));
+      at = id - before - (__shfl(upto, l, BH_WAVE) - __shfl(tiles, l, BH_WAVE));
     } else {
       before += __shfl(upto, 63, BH_WAVE);
     }
   }
-  if (expert < 0) return;      // beyond the last tile: the whole workgroup
   expert = __builtin_amdgcn_readfirstlane(expert);
   count = __builtin_amdgcn_readfirstlane(count);
   at = __builtin_amdgcn_readfirstlane(at);
   const int row_tiles = (count + ROWS - 1) / ROWS, p0 = (at % row_tiles) * ROWS, tile_n = at / row_tiles;
   const int32_t* pairs = list + (size_t)expert * capacity;
-  const uint8_t* ap[XB];
-  const uint8_t* wp[YB];
-  const float* ws[YB];
+  const uint8_t* from[Ring::EACH];
+  size_t row_at[Ring::A_EACH];
+#pragma unroll
+  for (int i = 0; i < Ring::A_EACH; ++i) {
+    const int piece = wave * Ring::A_EACH + i;
+    from[i] = a + piece % 2 * 64;
+    row_at[i] = (size_t)(pairs[min(p0 + piece / 2 * 16 + lane % 16, count - 1)] / in_div) * steps * F8_K + 16 * (lane / 16);
+  }
+#pragma unroll
+  for (int i = 0; i < Ring::W_EACH; ++i) {
+    const int piece = wave * Ring::W_EACH + i, b = piece / 2, column = b / YB, y = b % YB;
+    const int block = min((tile_n * WN + column) * HALF + y % HALF, blocks - 1);
+    from[Ring::A_EACH + i] = w.data + (((size_t)expert * Ring::G + y / HALF) * blocks + block) * steps * F8_BLOCK + piece % 2 * 1024;
+  }
   const uint32_t* xp[XB];
 #pragma unroll
-  for (int x = 0; x < XB; ++x) {
-    const int row = pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)] / in_div;
-    ap[x] = a + (size_t)row * stretches * F8_K + 16 * (lane / 16);
-    xp[x] = exponents + row;
-  }
+  for (int x = 0; x < XB; ++x) xp[x] = exponents + pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)] / in_div;
+  const float* ws[Ring::G];
 #pragma unroll
-  for (int y = 0; y < YB; ++y) {
-    const int block = min((tile_n * 2 + wn) * HALF + y % HALF, blocks - 1);
-    const long matrix = (long)expert * (GATED ? 2 : 1) + y / HALF;
-    wp[y] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
-    ws[y] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
-  }
+  for (int g = 0; g < Ring::G; ++g)
+    ws[g] = w.scales + (((size_t)expert * Ring::G + g) * w.scale_rows() + min((tile_n * WN + wn) * HALF, blocks - 1) / 8) * steps;
   f8_f32x4_t acc[XB][YB];
+  Ring::walk(ring, from, row_at, F8_K, xp, padded, ws, steps, acc);
+
+  int pair[XB];      // (read again: registers are short in the walk)
 #pragma unroll
-  for (int x = 0; x < XB; ++x)
+  for (int x = 0; x < XB; ++x) pair[x] = pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)];
+  if constexpr (GATED) {
+    uint32_t* largest = reinterpret_cast<uint32_t*>(ring);      // [wave column][row]
+    __syncthreads();      // every wave has read its last step
 #pragma unroll
-    for (int y = 0; y < YB; ++y) acc[x][y] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
-  f8_walk<FULL, XB, YB, F8_K, 64>(ap, xp, padded, wp, ws, 0, stretches, acc);
+    for (int x = 0; x < XB; ++x) {
+      const float wgt = in_weights ? in_weights[pair[x]] : 1.0f;
+      uint32_t most = 0;
 #pragma unroll
-  for (int x = 0; x < XB; ++x) {
-    const int p = p0 + (wm * XB + x) * 16 + lane % 16;
-    if (p >= count) continue;
-    const int pair = pairs[p];
-    const float wgt = GATED && in_weights ? in_weights[pair] : 1.0f;
+      for (int y = 0; y < HALF; ++y)
 #pragma unroll
-    for (int y = 0; y < HALF; ++y) {
-      const int n = ((tile_n * 2 + wn) * HALF + y) * 16 + 4 * (lane / 16);
+        for (int e = 0; e < 4; ++e) {
+          const int n = tile_n * OUTS + (wn * HALF + y) * 16 + 4 * (lane / 16) + e;
+          const float v = activated(acc[x][y][e] * wgt, acc[x][y + HALF][e] * wgt, gate);
+          acc[x][y][e] = n < N ? v : 0.f;
+          most = f8_larger(most, acc[x][y][e]);
+        }
+      most = f8_largest_of_row(most);
+      if (lane < 16) largest[wn * ROWS + (wm * XB + x) * 16 + lane] = most;
+    }
+    __syncthreads();
+    const int out_stretches = (N + F8_K - 1) / F8_K;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= w.rows) break;
-        out[(size_t)pair * w.rows + n + e] =
-            GATED ? activated(acc[x][y][e] * wgt, acc[x][y + (GATED ? HALF : 0)][e] * wgt, gate) : acc[x][y][e];
+    for (int x = 0; x < XB; ++x) {
+      const int r = (wm * XB + x) * 16 + lane % 16;
+      uint32_t most = largest[r];
+#pragma unroll
+      for (int column = 1; column < WN; ++column) most = max(most, largest[column * ROWS + r]);
+      const uint32_t exponent = f8_exponent(most);
+      if (p0 + r >= count) continue;
+      uint8_t* row = reinterpret_cast<uint8_t*>(out) + ((size_t)pair[x] * out_stretches + tile_n) * F8_K;
+#pragma unroll
+      for (int y = 0; y < HALF; ++y)
+        *reinterpret_cast<uint32_t*>(row + (wn * HALF + y) * 16 + 4 * (lane / 16)) =
+            f8_four(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3], f8_scale(exponent));
+      if (wn == 0 && lane < 16) out_exponents[((size_t)(tile_n / 4) * out_padded + pair[x]) * 4 + tile_n % 4] = (uint8_t)exponent;
+    }
+  } else {
+    const bool fours = N % 4 == 0;
+#pragma unroll
+    for (int x = 0; x < XB; ++x) {
+      if (p0 + (wm * XB + x) * 16 + lane % 16 >= count) continue;
+      float* row = reinterpret_cast<float*>(out) + (size_t)pair[x] * N;
+#pragma unroll
+      for (int y = 0; y < HALF; ++y) {
+        const int n = tile_n * OUTS + (wn * HALF + y) * 16 + 4 * (lane / 16);
+        if (n >= N) continue;
+        if (fours) {
+          store_four(row + n, acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) row[n + e] = acc[x][y][e];
+        }
       }
     }
   }
 }
 
 // ---- the sum over a row's pairs --------------------------------------------------------------------------------
-template <typename T, typename TC>
+// VN: neighbouring outputs of a thread (4: a multiple of 4 outputs).
+template <typename T, typename TC, int VN>
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float* __restrict__ y, const int32_t* __restrict__ chosen, const float* __restrict__ weights,
                                                           const T* __restrict__ through, TC* __restrict__ out, int E, int top, int D, int fresh) {
-  const int row = blockIdx.x, d = blockIdx.y * blockDim.x + threadIdx.x;
+  const int row = blockIdx.x, d = VN * (blockIdx.y * blockDim.x + threadIdx.x);
   if (d >= D) return;
-  float total = 0.f;
+  float total[VN] = {};
+#pragma unroll 4
   for (int j = 0; j < top; ++j) {
     const long pair = (long)row * top + j;
     const int e = chosen[pair];
     if (e < 0 || (e >= E && through == nullptr)) continue;
-    const float share = e >= E ? to_f32(through[(size_t)row * D + d]) : y[pair * D + d];
-    total = fmaf(weights ? weights[pair] : 1.0f, share, total);
+    const float f = weights ? weights[pair] : 1.0f;
+    if constexpr (VN == 4) {
+      const float4 share = e >= E ? load_four(through + (size_t)row * D + d) : load_four(y + pair * D + d);
+      total[0] = fmaf(f, share.x, total[0]), total[1] = fmaf(f, share.y, total[1]), total[2] = fmaf(f, share.z, total[2]), total[3] = fmaf(f, share.w, total[3]);
+    } else {
+      total[0] = fmaf(f, e >= E ? to_f32(through[(size_t)row * D + d]) : y[pair * D + d], total[0]);
+    }
   }
   TC* at = out + (size_t)row * D + d;
-  *at = from_f32<TC>(fresh ? total : to_f32(*at) + total);
+  if constexpr (VN == 4) {
+    if (!fresh) {
+      const float4 old = load_four(at);
+      total[0] += old.x, total[1] += old.y, total[2] += old.z, total[3] += old.w;
+    }
+    store_four(at, total[0], total[1], total[2], total[3]);
+  } else {
+    *at = from_f32<TC>(fresh ? total[0] : to_f32(*at) + total[0]);
+  }
 }
 
 }  // namespace
@@ -249,38 +321,55 @@ extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, con
   return bh_check_launch("experts_float8_rows");
 }
 
-// One of the two products of `tiles`, from rows in 8 bits; lists [E][capacity] and counts [E] as experts_group makes them.
+// One of the two products of `tiles`, from rows in 8 bits; lists [E][capacity] and counts [E] as experts_group makes them.  Gated: out is
+// rows in 8 bits [pairs], row after row, with their exponents.
 extern "C" int bh_experts_float8_tiles(const void* a, const void* exponents, int rows, int in_div, const int32_t* list, int capacity, const int32_t* counts,
-                                       int pairs, int E, const void* w, const void* scales, float* out, int N, int K, int gated, float limit, float alpha,
-                                       float shift, const float* in_weights, int full, hipStream_t stream) {
+                                       int pairs, int E, const void* w, const void* scales, void* out, void* out_exponents, int N, int K, int gated,
+                                       float limit, float alpha, float shift, const float* in_weights, int full, hipStream_t stream) {
   BH_REQUIRE(rows > 0 && pairs > 0 && E > 0 && N > 0 && K > 0 && in_div > 0 && capacity > 0, "experts_float8: sizes must be positive");
-  BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents | (uintptr_t)w) % 16 == 0, "experts_float8: rows and weights must be 16-byte aligned");
+  BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents | (uintptr_t)w | (uintptr_t)out) % 16 == 0, "experts_float8: rows and weights must be 16-byte aligned");
+  BH_REQUIRE(!gated || out_exponents != nullptr, "experts_float8: rows in 8 bits have exponents");
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
-  const int outs = gated ? 64 : 128;
-  const long most = (long)((N + outs - 1) / outs) * (pairs / 64 + (pairs < E ? pairs : E));      // every expert's last tile may be a part of one
+  const bool wide = pairs >= 64L * E;      // tiles of 128 pairs
+  const int outs = gated ? 128 : 256, tile = wide ? 128 : 64;
+  const long most = (long)((N + outs - 1) / outs) * (pairs / tile + (pairs < E ? pairs : E)) + 8;      // every expert's last tile may be a part of one
   BH_REQUIRE(most < (1L << 31), "experts_float8: %d pairs of %d outputs are too many", pairs, N);
   const ExpertGate gate = {limit, alpha, shift};
-#define BH_F8_TILES(GATED, FULL)                                                                                                                \
-  experts_tiles8_kernel<GATED, FULL><<<(unsigned)most, 256, 0, stream>>>((const uint8_t*)a, (const uint32_t*)exponents, (rows + 15) / 16 * 16, in_div, \
-                                                                        list, capacity, counts, E, weight, out, gate, in_weights)
+#define BH_F8_TILES(GATED, FULL, XB)                                                                                                            \
+  experts_ring_kernel<GATED, FULL, XB><<<(unsigned)most, 512, 0, stream>>>((const uint8_t*)a, (const uint32_t*)exponents, (rows + 15) / 16 * 16, in_div, \
+                                                                          list, capacity, counts, E, weight, out, (uint8_t*)out_exponents,      \
+                                                                          (pairs + 15) / 16 * 16, gate, in_weights)
+#define BH_F8_TILES_OF(GATED, FULL)          \
+  do {                                       \
+    if (wide) BH_F8_TILES(GATED, FULL, 4);   \
+    else BH_F8_TILES(GATED, FULL, 2);        \
+  } while (0)
   if (gated) {
-    if (full) BH_F8_TILES(true, true);
-    else BH_F8_TILES(true, false);
-  } else if (full) BH_F8_TILES(false, true);
-  else BH_F8_TILES(false, false);
+    if (full) BH_F8_TILES_OF(true, true);
+    else BH_F8_TILES_OF(true, false);
+  } else if (full) BH_F8_TILES_OF(false, true);
+  else BH_F8_TILES_OF(false, false);
+#undef BH_F8_TILES_OF
+#undef BH_F8_TILES
   return bh_check_launch("experts_float8_tiles");
 }
 
 extern "C" int bh_experts_float8_sum(const float* y, const int32_t* chosen, const float* weights, const void* through, int dtype, void* out, int c_dtype,
                                      int n_rows, int E, int top, int D, int fresh, hipStream_t stream) {
   BH_REQUIRE(n_rows > 0 && top > 0 && D > 0 && E > 0 && (D + 255) / 256 <= 65535, "experts_float8: %d rows of %d outputs", n_rows, D);
-  const dim3 grid(n_rows, (D + 255) / 256);
-#define BH_F8_SUM(T, TC) experts_sum_kernel<T, TC><<<grid, 256, 0, stream>>>(y, chosen, weights, (const T*)through, (TC*)out, E, top, D, fresh)
   BH_REQUIRE((dtype == BH_F32 || dtype == BH_BF16) && (c_dtype == BH_F32 || c_dtype == BH_BF16), "experts_float8: unknown dtype");
+  const bool fours = D % 4 == 0 && ((uintptr_t)y | (uintptr_t)through | (uintptr_t)out) % 16 == 0;
+  const dim3 grid(n_rows, (D / (fours ? 4 : 1) + 255) / 256);
+#define BH_F8_SUM(T, TC)                                                                                                                         \
+  do {                                                                                                                                           \
+    if (fours) experts_sum_kernel<T, TC, 4><<<grid, 256, 0, stream>>>(y, chosen, weights, (const T*)through, (TC*)out, E, top, D, fresh);         \
+    else experts_sum_kernel<T, TC, 1><<<grid, 256, 0, stream>>>(y, chosen, weights, (const T*)through, (TC*)out, E, top, D, fresh);               \
+  } while (0)
   if (dtype == BH_F32) {
     if (c_dtype == BH_F32) BH_F8_SUM(float, float);
     else BH_F8_SUM(float, bf16_t);
   } else if (c_dtype == BH_F32) BH_F8_SUM(bf16_t, float);
   else BH_F8_SUM(bf16_t, bf16_t);
+#undef BH_F8_SUM
   return bh_check_launch("experts_float8_sum");
 }

@@ -306,7 +306,7 @@ class KernelSizes:
             "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
             "bh_experts_float8_few": [i, i],
             "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
-            "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
+            "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, p, i, i, i, f, f, f, p, i, p],
             "bh_experts_float8_sum": [p, p, p, p, i, p, i, i, i, i, i, i, p],
         }
         for name, argtypes in table.items():
@@ -927,6 +927,11 @@ class HipKernels(KernelSizes):
         spread = w.scales.repeat_interleave(128, dim=1)[:, :w.rows].repeat_interleave(128, dim=2)[:, :, :cols]
         return (values[:, :w.rows, :cols].contiguous().view(torch.float8_e4m3fn).to(torch.float32) * spread).reshape(total, cols)
 
+    def _new_float8_rows(self, rows, width, in_rows) -> Float8Rows:
+        (data_bytes, exponent_bytes), words = Float8Rows.bytes_of(rows, width), -(-width // 512)
+        return Float8Rows(torch.empty(data_bytes, dtype=torch.uint8, device=self.device),
+                          torch.empty((words, exponent_bytes // 4 // words), dtype=torch.int32, device=self.device), rows, width, in_rows)
+
     def to_float8(self, x, gate=None, in_rows=False) -> Float8Rows:
         """The rows `x` [n, K] (float32 or bfloat16) as `Float8Rows`: a stretch of 128 columns of a row has the scale 2^e with the least
         e >= -126 for which no magnitude exceeds 448 * 2^e, a value is the nearest e4m3 of value / 2^e; a value that is not finite becomes NaN.
@@ -936,9 +941,7 @@ class HipKernels(KernelSizes):
         if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] % (2 if gate else 1):
             raise KernelError(f"to_float8: a matrix (of an even width with a gate), got {getattr(x, 'shape', type(x))}")
         rows, width = x.shape[0], x.shape[1] // (2 if gate else 1)
-        data_bytes, exponent_bytes = Float8Rows.bytes_of(rows, width)
-        out = Float8Rows(torch.empty(data_bytes, dtype=torch.uint8, device=self.device),
-                         torch.empty((-(-width // 512), exponent_bytes // 4 // -(-width // 512)), dtype=torch.int32, device=self.device), rows, width, in_rows)
+        out = self._new_float8_rows(rows, width, in_rows)
         self._check(self.lib.bh_float8_rows(self._ptr(x, "rows"), _code(x, "rows"), out.data.data_ptr(), out.exponents.data_ptr(), rows, width,
                                             int(out.in_rows), self.GATES[gate] if gate else 0, self._stream()))
         return out
@@ -1015,10 +1018,10 @@ class HipKernels(KernelSizes):
         act = (float(limit), float(alpha), float(shift))
         x_at, x_code, out_at, out_code = self._ptr(x, "experts x"), _code(x, "experts x"), self._ptr(out, "experts out"), _code(out, "experts out")
         through_at = self._ptr(through, "experts input", None, True)
-        inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
         y = torch.empty((pairs, width), dtype=torch.float32, device=self.device)
         in_weights = weights_at if weigh_input else None
         if lib.bh_experts_float8_few(pairs, experts):
+            inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
             self._check(lib.bh_experts_float8_rows(x_at, x_code, top, chosen_at, pairs, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(),
                                                    ff, k, 1, *act, in_weights, int(full_up), stream))
             self._check(lib.bh_experts_float8_rows(inner.data_ptr(), F32, 1, chosen_at, pairs, experts, w_down.data.data_ptr(), w_down.scales.data_ptr(),
@@ -1027,14 +1030,14 @@ class HipKernels(KernelSizes):
             lists = torch.empty((experts, pairs), dtype=torch.int32, device=self.device)      # a row may name an expert more than once
             counts = torch.empty((experts,), dtype=torch.int32, device=self.device)
             self._check(lib.bh_experts_group(chosen_at, pairs, lists.data_ptr(), pairs, counts.data_ptr(), experts, stream))
-            rows = self.to_float8(x, in_rows=True)
-            self._check(lib.bh_experts_float8_tiles(rows.data.data_ptr(), rows.exponents.data_ptr(), n, top, lists.data_ptr(), pairs, counts.data_ptr(), pairs,
-                                                    experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(), ff, k, 1, *act, in_weights,
-                                                    int(full_up), stream))
-            rows = self.to_float8(inner, in_rows=True)
-            self._check(lib.bh_experts_float8_tiles(rows.data.data_ptr(), rows.exponents.data_ptr(), pairs, 1, lists.data_ptr(), pairs, counts.data_ptr(), pairs,
-                                                    experts, w_down.data.data_ptr(), w_down.scales.data_ptr(), y.data_ptr(), width, ff, 0, *act, None,
-                                                    int(full), stream))
+            rows, inner = self.to_float8(x, in_rows=True), self._new_float8_rows(pairs, ff, True)
+            for a, in_rows, div, w, out_rows, out_exponents, outs, ins, is_full in (
+                    (rows, n, top, w_up, inner.data, inner.exponents, ff, k, full_up), (inner, pairs, 1, w_down, y, None, width, ff, full)):
+                gated = out_exponents is not None
+                self._check(lib.bh_experts_float8_tiles(
+                    a.data.data_ptr(), a.exponents.data_ptr(), in_rows, div, lists.data_ptr(), pairs, counts.data_ptr(), pairs, experts, w.data.data_ptr(),
+                    w.scales.data_ptr(), out_rows.data_ptr(), out_exponents.data_ptr() if gated else None, outs, ins, int(gated), *act,
+                    in_weights if gated else None, int(is_full), stream))
         self._check(lib.bh_experts_float8_sum(y.data_ptr(), chosen_at, None if weigh_input else weights_at, through_at, x_code, out_at, out_code, n, experts, top,
                                               width, int(bool(fresh)), stream))
 

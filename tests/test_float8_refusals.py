@@ -45,8 +45,8 @@ def test_experts_refuse(sizes):
     assert lib.bh_experts_float8_rows(AT, 0, 1, AT, 0, 4, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
     assert lib.bh_experts_float8_rows(AT, 0, 1, AT, 1 << 20, 4, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
     assert lib.bh_experts_float8_rows(AT, 9, 1, AT, 4, 4, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
-    assert lib.bh_experts_float8_tiles(AT, AT, 0, 1, AT, 4, AT, 4, 4, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
-    assert lib.bh_experts_float8_tiles(AT, AT, 4, 1, AT, 4, AT, 4, 4, AT + 1, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
+    assert lib.bh_experts_float8_tiles(AT, AT, 0, 1, AT, 4, AT, 4, 4, AT, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
+    assert lib.bh_experts_float8_tiles(AT, AT, 4, 1, AT, 4, AT, 4, 4, AT + 1, AT, AT, AT, 16, 128, 1, 1.0, 1.0, 0.0, None, 1, None) != 0
     assert lib.bh_experts_float8_sum(AT, AT, AT, None, 0, AT, 0, 0, 4, 1, 128, 1, None) != 0
     assert lib.bh_experts_float8_sum(AT, AT, AT, None, 3, AT, 0, 4, 4, 1, 128, 1, None) != 0
 
