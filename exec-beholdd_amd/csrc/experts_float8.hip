@@ -172,12 +172,12 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
   const int row_tiles = (count + ROWS - 1) / ROWS, p0 = (at % row_tiles) * ROWS, tile_n = at / row_tiles;
   const int32_t* pairs = list + (size_t)expert * capacity;
   const uint8_t* from[Ring::EACH];
-  size_t row_at[Ring::A_EACH];
+  uint32_t row_at[Ring::ROW_PARTS];
 #pragma unroll
   for (int i = 0; i < Ring::A_EACH; ++i) {
     const int piece = wave * Ring::A_EACH + i;
     from[i] = a + piece % 2 * 64;
-    row_at[i] = (size_t)(pairs[min(p0 + piece / 2 * 16 + lane % 16, count - 1)] / in_div) * steps * F8_K + 16 * (lane / 16);
+    row_at[i] = (uint32_t)(pairs[min(p0 + piece / 2 * 16 + lane % 16, count - 1)] / in_div) * (steps * F8_K) + 16 * (lane / 16);
   }
 #pragma unroll
   for (int i = 0; i < Ring::W_EACH; ++i) {
@@ -185,15 +185,15 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
     const int block = min((tile_n * WN + column) * HALF + y % HALF, blocks - 1);
     from[Ring::A_EACH + i] = w.data + (((size_t)expert * Ring::G + y / HALF) * blocks + block) * steps * F8_BLOCK + piece % 2 * 1024;
   }
-  const uint32_t* xp[XB];
+  uint32_t x_at[XB];
 #pragma unroll
-  for (int x = 0; x < XB; ++x) xp[x] = exponents + pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)] / in_div;
+  for (int x = 0; x < XB; ++x) x_at[x] = pairs[min(p0 + (wm * XB + x) * 16 + lane % 16, count - 1)] / in_div;
   const float* ws[Ring::G];
 #pragma unroll
   for (int g = 0; g < Ring::G; ++g)
     ws[g] = w.scales + (((size_t)expert * Ring::G + g) * w.scale_rows() + min((tile_n * WN + wn) * HALF, blocks - 1) / 8) * steps;
   f8_f32x4_t acc[XB][YB];
-  Ring::walk(ring, from, row_at, F8_K, xp, padded, ws, steps, acc);
+  Ring::walk(ring, from, row_at, F8_K, exponents, x_at, padded, ws, steps, acc);
 
   int pair[XB];      // (read again: registers are short in the walk)
 #pragma unroll
@@ -328,6 +328,7 @@ extern "C" int bh_experts_float8_tiles(const void* a, const void* exponents, int
                                        float limit, float alpha, float shift, const float* in_weights, int full, hipStream_t stream) {
   BH_REQUIRE(rows > 0 && pairs > 0 && E > 0 && N > 0 && K > 0 && in_div > 0 && capacity > 0, "experts_float8: sizes must be positive");
   BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents | (uintptr_t)w | (uintptr_t)out) % 16 == 0, "experts_float8: rows and weights must be 16-byte aligned");
+  BH_REQUIRE((long)(rows + 15) * ((K + 511) / 512 * 512) < (1L << 32), "experts_float8: %d rows of %d inputs do not lie within 4 GB", rows, K);
   BH_REQUIRE(!gated || out_exponents != nullptr, "experts_float8: rows in 8 bits have exponents");
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
   const bool wide = pairs >= 64L * E;      // tiles of 128 pairs

@@ -20,31 +20,40 @@
     __builtin_amdgcn_sched_barrier(0);    \
   } while (0)
 
-// FULL: float8.h.  G: matrices that a wave's weight rows are of (2: gate rows, then as many up rows).
-template <bool FULL_, int XB_, int YB_, int WM_, int WN_, int R_, int G_>
+#define F8_BUFFER 0x00020000      // a buffer of bytes; the addresses are checked by the launch
+
+// FULL: float8.h.  G: matrices that a wave's weight rows are of (2: gate rows, then as many up rows).  DIRECT: a wave loads its rows of the
+// next step from memory into its other set of registers itself, and only the weights go through LDS.
+template <bool FULL_, int XB_, int YB_, int WM_, int WN_, int R_, int G_, bool DIRECT_ = false>
 struct F8Ring {
-  static constexpr bool FULL = FULL_;
+  static constexpr bool FULL = FULL_, DIRECT = DIRECT_;
   static constexpr int XB = XB_, YB = YB_, WM = WM_, WN = WN_, R = R_, G = G_;
-  static constexpr int WAVES = WM * WN, A_PIECES = 2 * XB * WM, W_PIECES = 2 * YB * WN, PIECES = A_PIECES + W_PIECES;
+  static constexpr int WAVES = WM * WN, A_PIECES = DIRECT ? 0 : 2 * XB * WM, W_PIECES = 2 * YB * WN, PIECES = A_PIECES + W_PIECES;
   static constexpr int A_EACH = A_PIECES / WAVES, W_EACH = W_PIECES / WAVES, EACH = A_EACH + W_EACH, HALF = YB / G;
+  static constexpr int ROW_PARTS = DIRECT ? XB : A_EACH;      // addresses of rows that a wave has: of its blocks, or of its pieces
   static constexpr int ROWS = 16 * XB * WM, OUTS = 16 * HALF * WN;
-  static_assert(A_PIECES % WAVES == 0 && W_PIECES % WAVES == 0 && R >= 2 && EACH * (R - 2) < 64, "every wave brings as many pieces, and their count fits s_waitcnt");
+  static_assert(A_PIECES % WAVES == 0 && W_PIECES % WAVES == 0 && R >= 2 && EACH * (R - 2) < 64 && (!DIRECT || R >= 3), "every wave brings as many pieces, and their count fits s_waitcnt");
   static_assert(F8_K % (16 * HALF) == 0, "a wave's blocks of a matrix have one scale");
   static_assert(YB % 2 == 0 && YB % G == 0, "the first weights of a step lie in the first set");
 
-  // Where a wave's pieces come from: pieces 0 .. A_EACH - 1 of the rows, `row_step` bytes a step, the others of the weights.  `row_at`: a
-  // lane's own offset (16 * lane for rows in blocks).
+  // Where a wave's operands come from: the first ROW_PARTS addresses are those of rows, `row_step` bytes a step, the others those of its pieces
+  // of the weights; row_at: a lane's own offset (16 * lane for rows in blocks), x_at: that of its row's word of exponents, four stretches
+  // `exponents_step` words behind the four before.  All of an address but the lane's offset is the same for the wave: buffer loads take it from
+  // scalar registers, of which there are enough.  DIRECT takes rows in blocks.
   // acc[x][y][i]: row 16 (XB wm + x) + lane % 16 of the tile, weight row 16 y + 4 (lane / 16) + i of the wave's.
-  template <typename OFFSET>
-  __device__ static inline void walk(f8_u32x4_t* __restrict__ ring, const uint8_t* const (&from)[EACH], const OFFSET (&row_at)[A_EACH], int row_step,
-                                     const uint32_t* const (&xp)[XB], long exponents_step, const float* const (&ws)[G], int steps,
-                                     f8_f32x4_t (&acc)[XB][YB]) {
+  __device__ static inline void walk(f8_u32x4_t* __restrict__ ring, const uint8_t* const (&from)[ROW_PARTS + W_EACH], const uint32_t (&row_at)[ROW_PARTS],
+                                     int row_step, const uint32_t* exponents, const uint32_t (&x_at)[XB], uint32_t exponents_step,
+                                     const float* const (&ws)[G], int steps, f8_f32x4_t (&acc)[XB][YB]) {
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
+    __amdgpu_buffer_rsrc_t buffer[ROW_PARTS + W_EACH];
+#pragma unroll
+    for (int i = 0; i < ROW_PARTS + W_EACH; ++i) buffer[i] = __builtin_amdgcn_make_buffer_rsrc((void*)from[i], 0, -1, F8_BUFFER);
+    const __amdgpu_buffer_rsrc_t words_buffer = __builtin_amdgcn_make_buffer_rsrc((void*)exponents, 0, -1, F8_BUFFER);
     auto ask_piece = [&](int i, int step, int place) {
-      const uint8_t* at = i < A_EACH ? from[i] + (size_t)step * row_step + row_at[i < A_EACH ? i : 0] : from[i] + (size_t)step * F8_BLOCK + lane * 16;
       const int piece = i < A_EACH ? wave * A_EACH + i : A_PIECES + wave * W_EACH + i - A_EACH;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at,
-                                       (__attribute__((address_space(3))) void*)&ring[(place * PIECES + piece) * 64], 16, 0, 0);
+      __attribute__((address_space(3))) void* to = (__attribute__((address_space(3))) void*)&ring[(place * PIECES + piece) * 64];
+      if (i < A_EACH) __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer[i], to, 16, row_at[i < A_EACH ? i : 0], step * row_step, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer[ROW_PARTS + i - A_EACH], to, 16, lane * 16, step * F8_BLOCK, 0, 0);
     };
     auto ask_rows = [&](int step, int place) {
 #pragma unroll
@@ -61,6 +70,10 @@ struct F8Ring {
     f8_operand_t af[2][XB], wf[2];
     uint32_t words[XB];
     float wsv[G];
+    auto load_a = [&](int step, int x) {
+      return f8_operand(__builtin_amdgcn_raw_buffer_load_b128(buffer[x], row_at[x], step * row_step, 0),
+                        __builtin_amdgcn_raw_buffer_load_b128(buffer[x], row_at[x] + 1024, step * row_step, 0));
+    };
     auto read_a = [&](int place, int x) {
       const f8_u32x4_t* at = &ring[(place * PIECES + 2 * (wm * XB + x)) * 64 + lane];
       return f8_operand(at[0], at[64]);
@@ -71,19 +84,19 @@ struct F8Ring {
     };
     auto ask_scales = [&](int step) {
 #pragma unroll
-      for (int x = 0; x < XB; ++x) words[x] = xp[x][(size_t)(step / 4) * exponents_step];
+      for (int x = 0; x < XB; ++x) words[x] = __builtin_amdgcn_raw_buffer_load_b32(words_buffer, x_at[x] * 4, (uint32_t)(step / 4) * exponents_step * 4, 0);
 #pragma unroll
       for (int g = 0; g < G; ++g) wsv[g] = ws[g][step];
     };
     ask_scales(0);
     for (int j = 0; j < R && j < steps; ++j) {
-      ask_rows(j, j);
+      if (!DIRECT) ask_rows(j, j);
       if (j < R - 1) ask_weights(j, j);
     }
     F8_WAIT(0);
     F8_MEET();
 #pragma unroll
-    for (int x = 0; x < XB; ++x) af[0][x] = read_a(0, x);
+    for (int x = 0; x < XB; ++x) af[0][x] = DIRECT ? load_a(0, x) : read_a(0, x);
 
     int place = 0;      // of the step that is multiplied
     // STEADY: the rows of step j + R and the weights of step j + R - 1 exist, and what was asked for in the last R - 2 steps may still be
@@ -103,7 +116,11 @@ struct F8Ring {
 #pragma unroll
         for (int g = 0; g < G; ++g) s[g][x] = xs * wsv[g];
       }
-      if (j + 1 < steps) ask_scales(j + 1);
+      if (STEADY || j + 1 < steps) ask_scales(j + 1);      // (no branches while steady: sums would be kept across them and scaled behind all MFMAs)
+      if (DIRECT && (STEADY || j + 1 < steps)) {
+#pragma unroll
+        for (int x = 0; x < XB; ++x) af[1 - U][x] = load_a(j + 1, x);
+      }
       F8Operand<FULL> xo[XB];
 #pragma unroll
       for (int x = 0; x < XB; ++x) xo[x].set(af[U][x]);
@@ -113,7 +130,7 @@ struct F8Ring {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[x][y][e] = fmaf(sum[t % 3][e], s[y / HALF][x], acc[x][y][e]);
       };
-      if (!STEADY && j + R < steps) ask_rows(j + R, place);
+      if (!DIRECT && !STEADY && j + R < steps) ask_rows(j + R, place);
       if (!STEADY && j + R - 1 < steps) ask_weights(j + R - 1, left);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -122,7 +139,7 @@ struct F8Ring {
         if (y + 1 < YB) wf[(y + 1) % 2] = read_w(place, y + 1);
 #pragma unroll
         for (int x = 0; x < XB; ++x)
-          if (x * YB / XB == y) af[1 - U][x] = read_a(next, x);
+          if (!DIRECT && x * YB / XB == y) af[1 - U][x] = read_a(next, x);
         if (STEADY) {
 #pragma unroll
           for (int i = 0; i < EACH; ++i)
@@ -134,9 +151,10 @@ struct F8Ring {
         for (int x = 0; x < XB; ++x) {
           const int t = y * XB + x;
           sum[t % 3] = f8_stretch(wo, xo[x]);
+          __builtin_amdgcn_sched_barrier(0);      // the compiler would have every sum scaled behind its own MFMA, and wait for it
           if (t >= 2) scaled(t - 2);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
       scaled(XB * YB - 2);
       scaled(XB * YB - 1);

@@ -266,6 +266,7 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
                               int N, int K, int ldc, int gate, int full, void* scratch, hipStream_t stream) {
   if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
   BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
+  BH_REQUIRE((long)(M + 15) * ((K + 511) / 512) < (1L << 30), "gemm_float8: the exponents of %d rows of %d inputs do not lie within 4 GB", M, K);
   const int tile = float8_ring_tile(M, N, K, gate != 0, full != 0);
   if (tile >= 0)
     return float8_ring_launch(tile, (const uint8_t*)a, (const uint32_t*)exponents, {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K}, c,
