@@ -42,6 +42,13 @@ __device__ inline uint32_t f8_exponent(uint32_t largest) {
 }
 __device__ inline float f8_scale(uint32_t exponent) { return __builtin_bit_cast(float, exponent << 23); }
 
+// Four neighbouring outputs in one store, rounded by the conversion instruction (to nearest, ties to even).
+__device__ inline void f8_store_four(float* to, const float (&v)[4]) { store_four(to, v[0], v[1], v[2], v[3]); }
+__device__ inline void f8_store_four(bf16_t* to, const float (&v)[4]) {
+  const f8_bf16x2_t a = {(__bf16)v[0], (__bf16)v[1]}, b = {(__bf16)v[2], (__bf16)v[3]};
+  *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+
 // Four values as bytes of a word.
 __device__ inline uint32_t f8_four(float a, float b, float c, float d, float scale) {
   f8_s16x2_t v = {0, 0};

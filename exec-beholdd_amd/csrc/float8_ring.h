@@ -88,15 +88,25 @@ struct F8Ring {
 #pragma unroll
       for (int g = 0; g < G; ++g) wsv[g] = ws[g][step];
     };
+    // The first step alone is waited for: its rows, then its weights, then what comes after.
     ask_scales(0);
-    for (int j = 0; j < R && j < steps; ++j) {
+    if (!DIRECT) ask_rows(0, 0);
+    if (DIRECT) {
+#pragma unroll
+      for (int x = 0; x < XB; ++x) af[0][x] = load_a(0, x);
+    }
+    ask_weights(0, 0);
+    for (int j = 1; j < R && j < steps; ++j) {
       if (!DIRECT) ask_rows(j, j);
       if (j < R - 1) ask_weights(j, j);
     }
-    F8_WAIT(0);
+    if (steps > R) F8_WAIT(EACH * (R - 2) + A_EACH);      // (all of them were asked for)
+    else F8_WAIT(0);
     F8_MEET();
+    if (!DIRECT) {
 #pragma unroll
-    for (int x = 0; x < XB; ++x) af[0][x] = DIRECT ? load_a(0, x) : read_a(0, x);
+      for (int x = 0; x < XB; ++x) af[0][x] = read_a(0, x);
+    }
 
     int place = 0;      // of the step that is multiplied
     // STEADY: the rows of step j + R and the weights of step j + R - 1 exist, and what was asked for in the last R - 2 steps may still be
@@ -104,7 +114,7 @@ struct F8Ring {
     auto multiply = [&](int j, auto odd, auto steady) {
       constexpr int U = decltype(odd)::value;
       constexpr bool STEADY = decltype(steady)::value;
-      if (STEADY) F8_WAIT(EACH * (R - 2));
+      if (STEADY) F8_WAIT(EACH * (R - 2));      // (of the first step: its weights and the next rows, which were asked for before the others)
       else F8_WAIT(0);
       F8_MEET();
       wf[0] = read_w(place, 0);

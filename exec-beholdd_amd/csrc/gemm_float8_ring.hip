@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
           const float4 old = load_four(at);
           v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
         }
-        store_four(at, v[0], v[1], v[2], v[3]);
+        f8_store_four(at, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
