@@ -25,7 +25,7 @@ constexpr int FEW_WAVES = 8, FEW_PAIRS = 4096;      // pairs of a call at most
 
 // grid (blocks of 16 outputs, min(pairs, E)).  With at most E pairs a workgroup is a pair's, and the first pair of an expert does all of
 // that expert's; otherwise it is an expert's.  The list of the expert's pairs is made here, by a wave, in their order.
-template <typename T, bool GATED, bool FULL, bool WHOLE>
+template <typename T, bool GATED, bool FULL, int LOAD>
 __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __restrict__ in, int in_div, const int32_t* __restrict__ chosen, int pairs,
                                                                     int E, F8Weight w, float* __restrict__ out, int K, ExpertGate gate,
                                                                     const float* __restrict__ in_weights) {
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __
     float wsv[2][TT];
     F8Stretch<T> xv[2];
     auto ask = [&](int u, int j) {
-      f8_load_stretch<T, WHOLE>(xv[u], row, there, j * F8_K + 16 * q, K);
+      f8_load_stretch<T, LOAD>(xv[u], row, there, j * F8_K + 16 * q, K);
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
@@ -303,12 +303,12 @@ extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, con
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
   const dim3 grid(weight.blocks(), pairs < E ? pairs : E);
   BH_REQUIRE(grid.y <= 65535, "experts_float8: up to 65,535 experts");
-  const bool whole = K % 8 == 0 && (uintptr_t)in % 16 == 0;
+  const int load = f8_load_of(in, K);
   const ExpertGate gate = {limit, alpha, shift};
 #define BH_F8_EXPERTS(T, GATED, FULL)                                                                                                                   \
   do {                                                                                                                                                  \
-    if (whole) experts_few_kernel<T, GATED, FULL, true><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights); \
-    else experts_few_kernel<T, GATED, FULL, false><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights);      \
+    if (load == F8_EVEN) experts_few_kernel<T, GATED, FULL, F8_EVEN><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights); \
+    else experts_few_kernel<T, GATED, FULL, F8_VALUES><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights);      \
   } while (0)
 #define BH_F8_EXPERTS_OF(T)                                                                                \
   do {                                                                                                     \

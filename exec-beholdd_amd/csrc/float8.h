@@ -71,6 +71,18 @@ __device__ inline uint32_t f8_larger_pair(uint32_t largest, uint32_t pair) {
 }
 __device__ inline uint32_t f8_of_pair(uint32_t pair) { return max(pair & 0xffffu, pair >> 16) << 16; }
 
+// What `join` makes of the values of a lane and of those 16, 32 and 48 lanes on (the four lanes of a row of an operand), for each of them.
+template <typename JOIN>
+__device__ inline uint32_t f8_over_rows(uint32_t v, JOIN join) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = join((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return join((uint32_t)b[0], (uint32_t)b[1]);
+}
+__device__ inline uint32_t f8_largest_of_row(uint32_t v) {
+  return f8_over_rows(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
 // A block's operand as it lies: a lane's two halves of 16 bytes.
 __device__ inline f8_operand_t f8_operand(f8_u32x4_t a, f8_u32x4_t b) {
   return f8_operand_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};

@@ -2,14 +2,6 @@
 #pragma once
 #include "float8.h"
 
-// The largest over the four lanes of a row (lane % 16).
-__device__ inline uint32_t f8_largest_of_row(uint32_t v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max((uint32_t)a[0], (uint32_t)a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return max((uint32_t)b[0], (uint32_t)b[1]);
-}
-
 // A lane's 32 values of a stretch of one row: k 16 q .. + 15 and 64 + 16 q .. + 15.
 template <typename T>
 struct F8Stretch;
@@ -48,24 +40,42 @@ struct F8Stretch<float> {
   }
 };
 
-// WHOLE: rows on addresses of 16 bytes whose K is a multiple of 8; otherwise value by value.
-template <typename T, bool WHOLE>
+// Rows that are in 8 bits already, in blocks.
+template <>
+struct F8Stretch<uint8_t> {
+  f8_u32x4_t v[2];
+  uint32_t exponent;
+  __device__ inline f8_operand_t quantised(float* scale) const {
+    *scale = f8_scale(exponent);
+    return f8_operand(v[0], v[1]);
+  }
+};
+
+// How a row's values are loaded.  EVEN: rows on addresses of 16 bytes, of whole stretches; a lane without a row of its own loads another
+// row's, whose outputs nobody stores.  PIECES: rows on addresses of 16 bytes whose K is a multiple of 8.  VALUES: any.
+enum F8Load { F8_VALUES = 0, F8_PIECES = 1, F8_EVEN = 2 };
+template <typename T, int LOAD>
 __device__ inline void f8_load_stretch(F8Stretch<T>& to, const T* __restrict__ row, bool there, int k0, int K) {
   constexpr int PIECE = 16 / sizeof(T), PIECES = 32 / PIECE;      // values of a load, loads of a lane
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int k = k0 + (i / (PIECES / 2)) * 64 + (i % (PIECES / 2)) * PIECE;
-    f8_u32x4_t piece = {0u, 0u, 0u, 0u};
-    if constexpr (WHOLE) {
-      if (there && k < K) piece = *reinterpret_cast<const f8_u32x4_t*>(row + k);
-    } else if (there) {
+    if constexpr (LOAD == F8_EVEN) {
+      to.v[i] = *reinterpret_cast<const f8_u32x4_t*>(row + k);
+    } else {
+      f8_u32x4_t piece = {0u, 0u, 0u, 0u};
+      if constexpr (LOAD == F8_PIECES) {
+        if (there && k < K) piece = *reinterpret_cast<const f8_u32x4_t*>(row + k);
+      } else if (there) {
 #pragma unroll
-      for (int j = 0; j < PIECE; ++j)
-        if (k + j < K) {
-          if constexpr (sizeof(T) == 4) piece[j] = __builtin_bit_cast(uint32_t, (float)row[k + j]);
-          else piece[j / 2] |= (uint32_t)row[k + j].bits << (16 * (j % 2));
-        }
+        for (int j = 0; j < PIECE; ++j)
+          if (k + j < K) {
+            if constexpr (sizeof(T) == 4) piece[j] = __builtin_bit_cast(uint32_t, (float)row[k + j]);
+            else piece[j / 2] |= (uint32_t)row[k + j].bits << (16 * (j % 2));
+          }
+      }
+      to.v[i] = piece;
     }
-    to.v[i] = piece;
   }
 }
+inline int f8_load_of(const void* rows, int K) { return (uintptr_t)rows % 16 != 0 || K % 8 != 0 ? F8_VALUES : K % F8_K == 0 ? F8_EVEN : F8_PIECES; }

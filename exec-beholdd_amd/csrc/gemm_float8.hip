@@ -1,6 +1,7 @@
 // Matrix products with weights and activations in 8 bits (float8.h): C[M, N] (+)= x[M, K] * W[N, K]^T, plain or gated.
-//   few     up to 32 rows, straight from bfloat16 or float32 rows: a wave quantises the stretch it multiplies
-//   tiles   any number of rows, from rows in 8 bits (float8_rows.hip), K in parts where the tiles alone leave compute units idle
+//   few     up to 32 rows straight from bfloat16 or float32 rows (a wave quantises the stretch it multiplies), up to 64 from rows in 8 bits
+//   tiles   from rows in 8 bits (float8_rows.hip), K in parts where the tiles alone leave compute units idle
+//   rings   many rows (gemm_float8_ring.hip)
 #include "float8_few.h"
 #include "float8_tiles.h"
 #include "gemm_float8_ring.h"
@@ -8,42 +9,65 @@
 namespace {
 
 // ---- a few rows ------------------------------------------------------------------------------------------------
-// Bound by reading W once.  A workgroup owns NT blocks of 16 weight rows (gated: as many pairs of gate and up); its eight waves take the
-// stretches of k in turn, each with the next one on its way, and quantise the rows' stretch themselves: 16 values a lane and half an
-// operand, the largest of a stretch found between the four lanes of a row.  The waves' sums are added through LDS in a fixed order.
+// Bound by reading W once, and for small W by the chain of a launch.  A workgroup owns `span` weight rows (gated: 16 pairs of gate and up);
+// its eight waves take the stretches of k in turn, each with DEPTH of them on their way, and quantise the rows' stretch themselves (16 values
+// a lane and half an operand, the largest of a stretch found between the four lanes of a row), or, from 33 rows on, read it in 8 bits.  The
+// waves' sums are added through LDS in a fixed order.
+// `span` is 16, a block of the layout; 24 where blocks of 16 are more than the compute units and fewer than twice as many, which would
+// leave some with two blocks and the others with one; 8 where they are half of the compute units or fewer.
 constexpr int FEW_WAVES = 8;
 
-// grid (ceil(blocks of W / NT)).  MB: blocks of 16 rows.  TC: the output's type.
-template <typename T, typename TC, int MB, int NT, bool GATED, bool FULL, bool WHOLE>
-__global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict__ x, F8Weight w, TC* __restrict__ c, int M, int K, int ldc,
-                                                             int accumulate, GateForm form) {
-  constexpr int TT = NT * (GATED ? 2 : 1);
+// grid (ceil(rows of W / span)).  MB: blocks of 16 rows.  NB: blocks of W that a span touches; MASKED: it is not the whole of one.  TC: the
+// output's type.  T: the rows' type (uint8_t: in 8 bits, in blocks, with their exponents).
+template <typename T, typename TC, int MB, int NB, bool GATED, bool FULL, int LOAD, bool MASKED, int DEPTH>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict__ x, const uint32_t* __restrict__ exponents, F8Weight w,
+                                                             TC* __restrict__ c, int M, int K, int ldc, int accumulate, int span, GateForm form) {
+  constexpr int TT = NB * (GATED ? 2 : 1);
   __shared__ float partial[FEW_WAVES][TT][MB][256];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int i = lane % 16, q = lane / 16, blocks = w.blocks(), stretches = w.stretches;
+  const int i = lane % 16, q = lane / 16, blocks = w.blocks(), stretches = w.stretches, left = (stretches - wave + FEW_WAVES - 1) / FEW_WAVES;
+  const int first_row = (int)blockIdx.x * span, first_block = first_row / 16;
+  int lo[NB], hi[NB];      // the rows of each block that this workgroup owns
+  int place[NB];           // a lane's place in it: where it has no row of its own that of the nearest, which brings no line more and is not stored
   const uint8_t* wp[TT];
   const float* ws[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int block = min((int)blockIdx.x * NT + t % NT, blocks - 1);      // (one beyond the last repeats it and stores nothing)
-    const int matrix = t / NT;
-    wp[t] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    const int block = min(first_block + t % NB, blocks - 1), matrix = t / NB;      // (one beyond the last repeats it)
+    wp[t] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK;
     ws[t] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+  }
+#pragma unroll
+  for (int t = 0; t < NB; ++t) {
+    const int row = (first_block + t) * 16;
+    lo[t] = MASKED ? max(first_row - row, 0) : 0;
+    hi[t] = MASKED ? min(min(first_row + span, w.rows) - row, 16) : 16;
+    place[t] = 16 * (MASKED ? 16 * q + max(min(i, hi[t] - 1), min(lo[t], 15)) : lane);
   }
   f8_f32x4_t acc[TT][MB];
 #pragma unroll
   for (int t = 0; t < TT; ++t)
 #pragma unroll
     for (int b = 0; b < MB; ++b) acc[t][b] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
-  f8_u32x4_t wv[2][TT][2];
-  float wsv[2][TT];
-  F8Stretch<T> xv[2][MB];
-  auto ask = [&](int u, int j) {
+  f8_u32x4_t wv[DEPTH][TT][2];
+  float wsv[DEPTH][TT];
+  F8Stretch<T> xv[DEPTH][MB];
+  auto ask = [&](int u, int n) {      // the wave's n-th stretch
+    const int j = wave + n * FEW_WAVES;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) f8_load_stretch<T, WHOLE>(xv[u][b], x + (size_t)min(b * 16 + i, M - 1) * K, b * 16 + i < M, j * F8_K + 16 * q, K);
+    for (int b = 0; b < MB; ++b) {
+      if constexpr (sizeof(T) == 1) {
+        const int row_blocks = (M + 15) / 16, block = min(b, row_blocks - 1);
+        const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(x + ((size_t)block * stretches + j) * F8_BLOCK + lane * 16);
+        xv[u][b].v[0] = from[0], xv[u][b].v[1] = from[64];
+        xv[u][b].exponent = (exponents[(size_t)(j / 4) * (row_blocks * 16) + block * 16 + i] >> (8 * (j % 4))) & 0xffu;
+      } else {
+        f8_load_stretch<T, LOAD>(xv[u][b], x + (size_t)min(b * 16 + i, M - 1) * K, b * 16 + i < M, j * F8_K + 16 * q, K);
+      }
+    }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
+      const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK + place[t % NB]);
       wv[u][t][0] = __builtin_nontemporal_load(from);
       wv[u][t][1] = __builtin_nontemporal_load(from + 64);
       wsv[u][t] = ws[t][j];
@@ -67,14 +91,16 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict
       }
     }
   };
-  int j = wave;
-  if (j < stretches) ask(0, j);
-  for (; j < stretches; j += 2 * FEW_WAVES) {
-    if (j + FEW_WAVES < stretches) ask(1, j + FEW_WAVES);
-    multiply(0);
-    if (j + 2 * FEW_WAVES < stretches) ask(0, j + 2 * FEW_WAVES);
-    if (j + FEW_WAVES < stretches) multiply(1);
-  }
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u)
+    if (u < left) ask(u, u);
+  for (int n = 0; n < left; n += DEPTH)
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (n + u < left) {
+        multiply(u);
+        if (n + u + DEPTH < left) ask(u, n + u + DEPTH);
+      }
 #pragma unroll
   for (int t = 0; t < TT; ++t)
 #pragma unroll
@@ -84,15 +110,15 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict
     const int b = e / 256, m = b * 16 + (e % 256) / 16, column = e % 16;
     if (m >= M) continue;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int n = ((int)blockIdx.x * NT + t) * 16 + column;
-      if (n >= w.rows) continue;
+    for (int t = 0; t < NB; ++t) {
+      const int n = (first_block + t) * 16 + column;
+      if (n >= w.rows || column < lo[t] || column >= hi[t]) continue;
       float sum[GATED ? 2 : 1];
 #pragma unroll
       for (int g = 0; g < (GATED ? 2 : 1); ++g) {
         sum[g] = 0.f;
 #pragma unroll
-        for (int v = 0; v < FEW_WAVES; ++v) sum[g] += partial[v][g * NT + t][b][e % 256];
+        for (int v = 0; v < FEW_WAVES; ++v) sum[g] += partial[v][g * NB + t][b][e % 256];
       }
       TC* at = c + (size_t)m * ldc + n;
       float value = GATED ? gate_mul(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
@@ -179,7 +205,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS = 32, MOST_PARTS = 16;
+constexpr int FEW_ROWS = 32, FEW_ROWS_IN_8 = 64, MOST_PARTS = 16;
 
 int parts_of(int M, int N, int K, bool gated) {
   const long tiles = (long)((M + 63) / 64) * ((N + (gated ? 63 : 127)) / (gated ? 64 : 128));
@@ -190,16 +216,50 @@ int parts_of(int M, int N, int K, bool gated) {
   return wanted < most ? wanted : most > 1 ? most : 1;
 }
 
+int span_of(int N, int K, bool gated) {
+  if (gated) return 16;
+  const int blocks = (N + 15) / 16, units = bh_compute_units();
+  if (2 * blocks <= units && K >= 1536) return 8;
+  if (blocks > units && blocks < 2 * units && (N + 23) / 24 <= units) return 24;
+  return 16;
+}
+
+template <typename T, typename TC, bool GATED, bool FULL, int MB>
+void launch_few_blocks(const void* x, const uint32_t* exponents, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
+  const int load = sizeof(T) == 1 ? (int)F8_EVEN : f8_load_of(x, K);
+  constexpr bool SPANS = sizeof(T) <= 2 && !GATED;      // (float32 rows go in whole blocks: they are not what a step of few rows has as a rule)
+  const int span = SPANS && load == F8_EVEN ? span_of(w.rows, K, GATED) : 16;
+  const dim3 grid((w.rows + span - 1) / span);
+#define BH_F8_FEW(NB, LOAD, MASKED, DEPTH)                                                                                            \
+  few_kernel<T, TC, MB, NB, GATED, FULL, LOAD, MASKED, DEPTH><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)x, exponents, w, c, M, K, \
+                                                                                                   ldc, accumulate, span, form)
+  constexpr int DEPTH = MB == 1 && !GATED ? 4 : MB <= 2 && sizeof(T) <= 2 ? 3 : 2;
+  if constexpr (SPANS) {
+    if (span == 8) {
+      BH_F8_FEW(1, F8_EVEN, true, DEPTH);
+      return;
+    }
+    if (span == 24) {
+      BH_F8_FEW(2, F8_EVEN, true, (MB == 1 ? 4 : 2));
+      return;
+    }
+  }
+  if (load == F8_EVEN) BH_F8_FEW(1, F8_EVEN, false, DEPTH);
+  else if constexpr (sizeof(T) != 1) {
+    if (load == F8_PIECES) BH_F8_FEW(1, F8_PIECES, false, 2);
+    else BH_F8_FEW(1, F8_VALUES, false, 2);
+  }
+#undef BH_F8_FEW
+}
+
 template <typename T, typename TC, bool GATED, bool FULL>
-void launch_few(const void* x, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
-  const bool whole = K % 8 == 0 && (uintptr_t)x % 16 == 0;
-  const dim3 grid(w.blocks());
-#define BH_F8_FEW(MB, WHOLE) few_kernel<T, TC, MB, 1, GATED, FULL, WHOLE><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)x, w, c, M, K, ldc, accumulate, form)
-  if (M <= 16) {
-    if (whole) BH_F8_FEW(1, true);
-    else BH_F8_FEW(1, false);
-  } else if (whole) BH_F8_FEW(2, true);
-  else BH_F8_FEW(2, false);
+void launch_few(const void* x, const uint32_t* exponents, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
+#define BH_F8_FEW(MB) launch_few_blocks<T, TC, GATED, FULL, MB>(x, exponents, w, c, M, K, ldc, accumulate, form, stream)
+  if constexpr (sizeof(T) == 1) {
+    if (M <= 48) BH_F8_FEW(3);
+    else BH_F8_FEW(4);
+  } else if (M <= 16) BH_F8_FEW(1);
+  else BH_F8_FEW(2);
 #undef BH_F8_FEW
 }
 
@@ -230,7 +290,7 @@ int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int 
 extern "C" int bh_gemm_float8_takes_rows(int M) { return M <= FEW_ROWS; }
 // Bytes of scratch memory of a product from rows in 8 bits.
 extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full) {
-  if (M <= 0 || N <= 0 || K <= 0 || float8_ring_tile(M, N, K, gated != 0, full != 0) >= 0) return 0;
+  if (M <= FEW_ROWS_IN_8 || N <= 0 || K <= 0 || float8_ring_tile(M, N, K, gated != 0, full != 0) >= 0) return 0;
   const int parts = parts_of(M, N, K, gated != 0);
   return parts > 1 ? (long)parts * M * N * (gated ? 2 : 1) * 4 : 0;
 }
@@ -254,8 +314,8 @@ extern "C" int bh_gemm_float8_few(const void* x, int dtype, const void* w, const
   const GateForm form = bh_gate_form(gate);
 #define BH_F8_RUN(TC, GATED, FULL)                                                                                     \
   do {                                                                                                                 \
-    if (dtype == BH_F32) launch_few<float, TC, GATED, FULL>(x, weight, (TC*)c, M, K, ldc, accumulate, form, stream);   \
-    else launch_few<bf16_t, TC, GATED, FULL>(x, weight, (TC*)c, M, K, ldc, accumulate, form, stream);                  \
+    if (dtype == BH_F32) launch_few<float, TC, GATED, FULL>(x, nullptr, weight, (TC*)c, M, K, ldc, accumulate, form, stream);   \
+    else launch_few<bf16_t, TC, GATED, FULL>(x, nullptr, weight, (TC*)c, M, K, ldc, accumulate, form, stream);                  \
   } while (0)
   BH_F8_BY_TYPES(BH_F8_RUN);
 #undef BH_F8_RUN
@@ -267,6 +327,14 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
   if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
   BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
   BH_REQUIRE((long)(M + 15) * ((K + 511) / 512) < (1L << 30), "gemm_float8: the exponents of %d rows of %d inputs do not lie within 4 GB", M, K);
+  if (M <= FEW_ROWS_IN_8) {
+    const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+    const GateForm form = bh_gate_form(gate);
+#define BH_F8_RUN(TC, GATED, FULL) launch_few<uint8_t, TC, GATED, FULL>(a, (const uint32_t*)exponents, weight, (TC*)c, M, K, ldc, accumulate, form, stream)
+    BH_F8_BY_TYPES(BH_F8_RUN);
+#undef BH_F8_RUN
+    return bh_check_launch("gemm_float8");
+  }
   const int tile = float8_ring_tile(M, N, K, gate != 0, full != 0);
   if (tile >= 0)
     return float8_ring_launch(tile, (const uint8_t*)a, (const uint32_t*)exponents, {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K}, c,
