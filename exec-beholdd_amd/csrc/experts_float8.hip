@@ -21,105 +21,241 @@ __device__ inline float activated(float g, float u, const ExpertGate& gate) {
 }
 
 // ---- few -------------------------------------------------------------------------------------------------------
-constexpr int FEW_WAVES = 8, FEW_PAIRS = 4096;      // pairs of a call at most
+// Bound by reading the matrices of the experts that have pairs.  A workgroup is one expert's and owns 8 / KS blocks of 16 outputs (gated: of
+// gate and up rows); KS waves share a block and take its stretches of k in turn, their sums added through LDS in a fixed order.  The rows of
+// up to 16 of the expert's pairs are brought into 8 bits once for the workgroup and kept in LDS, F8_SEGMENT stretches of k at a time, while
+// the first weights are on their way.
+constexpr int FEW_WAVES = 8, FEW_PAIRS = 1024;      // pairs of a call at most
+constexpr int FEW_TOP = 32;                         // pairs of a row, where the second product sums them itself
+constexpr int SEGMENT = 32;                         // stretches of the rows that LDS holds
 
-// grid (blocks of 16 outputs, min(pairs, E)).  With at most E pairs a workgroup is a pair's, and the first pair of an expert does all of
-// that expert's; otherwise it is an expert's.  The list of the expert's pairs is made here, by a wave, in their order.
-template <typename T, bool GATED, bool FULL, int LOAD>
+// grid (ceil(blocks / (8 / KS)), min(pairs, E)).  With at most E pairs a workgroup is a pair's, and the first pair of an expert does all of
+// that expert's; otherwise it is an expert's.  The list of the expert's pairs is made here, in their order.
+template <typename T, bool GATED, bool FULL, int LOAD, int KS, int DEPTH>
 __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __restrict__ in, int in_div, const int32_t* __restrict__ chosen, int pairs,
                                                                     int E, F8Weight w, float* __restrict__ out, int K, ExpertGate gate,
                                                                     const float* __restrict__ in_weights) {
-  constexpr int TT = GATED ? 2 : 1;
-  __shared__ float partial[FEW_WAVES][TT][256];
+  constexpr int TT = GATED ? 2 : 1, OWN = FEW_WAVES / KS;
+  extern __shared__ __attribute__((aligned(16))) f8_u32x4_t rows8[];      // [stretch of the segment][half][lane], then a scale for each stretch and row
+  __shared__ float partial[KS > 1 ? FEW_WAVES : 1][TT][256];
   __shared__ int mine[FEW_PAIRS];
-  __shared__ int found;
+  __shared__ int of_wave[FEW_WAVES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, i = lane % 16, q = lane / 16;
   const int expert = pairs <= E ? chosen[blockIdx.y] : (int)blockIdx.y;
   if (expert < 0 || expert >= E) return;      // the whole workgroup
-  if (wave == 0) {
-    int count = 0;
-    for (int p0 = 0; p0 < pairs; p0 += 64) {
-      const bool is = p0 + lane < pairs && chosen[min(p0 + lane, pairs - 1)] == expert;
-      const unsigned long long mask = __ballot(is);
-      if (is) mine[count + __popcll(mask & ((1ull << lane) - 1ull))] = p0 + lane;
-      count += __popcll(mask);
-    }
-    if (lane == 0) found = count;
-  }
-  __syncthreads();
-  const int count = found;
-  if (count == 0 || (pairs <= E && mine[0] != (int)blockIdx.y)) return;
-  const int block = blockIdx.x, blocks = w.blocks(), stretches = w.stretches;
+  const int blocks = w.blocks(), stretches = w.stretches, block = (int)blockIdx.x * OWN + wave / KS, share = wave % KS;
   const uint8_t* wp[TT];
   const float* ws[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const long matrix = (long)expert * TT + t;
-    wp[t] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
-    ws[t] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
+    const size_t matrix = (size_t)expert * TT + t;
+    const int b = min(block, blocks - 1);      // (one beyond the last repeats it and stores nothing)
+    wp[t] = w.data + (matrix * blocks + b) * stretches * F8_BLOCK + lane * 16;
+    ws[t] = w.scales + (matrix * w.scale_rows() + b / 8) * stretches;
   }
+  f8_u32x4_t wv[DEPTH][TT][2];
+  float wsv[DEPTH][TT];
+  auto ask = [&](int u, int j) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
+      wv[u][t][0] = from[0], wv[u][t][1] = from[64];
+      wsv[u][t] = ws[t][j];
+    }
+  };
+  auto ask_first = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (share + u * KS < min(stretches - j0, SEGMENT)) ask(u, j0 + share + u * KS);
+  };
+  ask_first(0);      // (the pairs are found while they are on their way)
+  // the pairs in pieces of 64, FEW_PAIRS / 512 neighbouring pieces a wave
+  constexpr int PIECES = FEW_PAIRS / 64 / FEW_WAVES;
+  unsigned long long masks[PIECES];
+  int own = 0;
+#pragma unroll
+  for (int u = 0; u < PIECES; ++u) {
+    const int p = (wave * PIECES + u) * 64 + lane;
+    masks[u] = __ballot(p < pairs && chosen[min(p, pairs - 1)] == expert);
+    own += __popcll(masks[u]);
+  }
+  if (lane == 0) of_wave[wave] = own;
+  __syncthreads();
+  int count = 0, at = 0;
+#pragma unroll
+  for (int v = 0; v < FEW_WAVES; ++v) {
+    if (v < wave) at += of_wave[v];
+    count += of_wave[v];
+  }
+#pragma unroll
+  for (int u = 0; u < PIECES; ++u) {
+    if (masks[u] >> lane & 1ull) mine[at + __popcll(masks[u] & ((1ull << lane) - 1ull))] = (wave * PIECES + u) * 64 + lane;
+    at += __popcll(masks[u]);
+  }
+  __syncthreads();
+  if (count == 0 || (pairs <= E && mine[0] != (int)blockIdx.y)) return;
+
+  const int segment = min(stretches, SEGMENT);
+  float* const scales8 = reinterpret_cast<float*>(rows8 + segment * 128);
   for (int p0 = 0; p0 < count; p0 += 16) {
-    const bool there = p0 + i < count;
     const T* row = in + (size_t)(mine[min(p0 + i, count - 1)] / in_div) * K;
     f8_f32x4_t acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
-    f8_u32x4_t wv[2][TT][2];
-    float wsv[2][TT];
-    F8Stretch<T> xv[2];
-    auto ask = [&](int u, int j) {
-      f8_load_stretch<T, LOAD>(xv[u], row, there, j * F8_K + 16 * q, K);
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
-        wv[u][t][0] = from[0], wv[u][t][1] = from[64];
-        wsv[u][t] = ws[t][j];
+    for (int j0 = 0; j0 < stretches; j0 += SEGMENT) {
+      const int here = min(stretches - j0, SEGMENT), left = (here - share + KS - 1) / KS;
+      if (p0 || j0) {
+        ask_first(j0);
+        __syncthreads();      // everyone has read what stood there
       }
-    };
-    auto multiply = [&](int u) {
-      F8Operand<FULL> xo;
-      float xs;
-      xo.set(xv[u].quantised(&xs));
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        F8Operand<FULL> wo;
-        wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
-        const f8_f32x4_t sum = f8_stretch(wo, xo);
-        const float s = xs * wsv[u][t];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sum[e], s, acc[t][e]);
+      for (int j = wave; j < here; j += FEW_WAVES) {
+        F8Stretch<T> x;
+        f8_load_stretch<T, LOAD>(x, row, true, (j0 + j) * F8_K + 16 * q, K);
+        float scale;
+        const f8_operand_t v = x.quantised(&scale);
+        rows8[j * 128 + lane] = f8_u32x4_t{(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]};
+        rows8[j * 128 + 64 + lane] = f8_u32x4_t{(uint32_t)v[4], (uint32_t)v[5], (uint32_t)v[6], (uint32_t)v[7]};
+        if (q == 0) scales8[j * 16 + i] = scale;
       }
-    };
-    int j = wave;
-    if (j < stretches) ask(0, j);
-    for (; j < stretches; j += 2 * FEW_WAVES) {
-      if (j + FEW_WAVES < stretches) ask(1, j + FEW_WAVES);
-      multiply(0);
-      if (j + 2 * FEW_WAVES < stretches) ask(0, j + 2 * FEW_WAVES);
-      if (j + FEW_WAVES < stretches) multiply(1);
+      __syncthreads();
+      for (int n = 0; n < left; n += DEPTH)
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u)
+          if (n + u < left) {
+            const int j = share + (n + u) * KS;
+            F8Operand<FULL> xo, wo;
+            xo.set(f8_operand(rows8[j * 128 + lane], rows8[j * 128 + 64 + lane]));
+            const float xs = scales8[j * 16 + i];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+              wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
+              const f8_f32x4_t sum = f8_stretch(wo, xo);
+              const float s = xs * wsv[u][t];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sum[e], s, acc[t][e]);
+            }
+            if (n + u + DEPTH < left) ask(u, j0 + j + DEPTH * KS);
+          }
     }
-    if (p0) __syncthreads();      // the sums of the pairs before have been read
+    if constexpr (KS > 1) {
+      __syncthreads();      // (the sums of the pairs before have been read)
 #pragma unroll
-    for (int t = 0; t < TT; ++t) *reinterpret_cast<f8_f32x4_t*>(&partial[wave][t][i * 16 + 4 * q]) = acc[t];
-    __syncthreads();
-    const int e = threadIdx.x, m = e / 16, n = block * 16 + e % 16;
-    if (e < 256 && p0 + m < count && n < w.rows) {
-      const int pair = mine[p0 + m];
-      float sum[TT];
+      for (int t = 0; t < TT; ++t) *reinterpret_cast<f8_f32x4_t*>(&partial[wave][t][i * 16 + 4 * q]) = acc[t];
+      __syncthreads();
+    }
+    if (share == 0 && block < blocks && p0 + i < count) {
+      const int pair = mine[p0 + i];
+      if constexpr (KS > 1) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        sum[t] = 0.f;
+        for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int v = 0; v < FEW_WAVES; ++v) sum[t] += partial[v][t][e];
+          for (int v = 1; v < KS; ++v) acc[t] += *reinterpret_cast<const f8_f32x4_t*>(&partial[wave + v][t][i * 16 + 4 * q]);
       }
-      if constexpr (GATED) {
-        const float wgt = in_weights ? in_weights[pair] : 1.0f;
-        out[(size_t)pair * w.rows + n] = activated(sum[0] * wgt, sum[TT - 1] * wgt, gate);
+      float v[4];
+      const float wgt = GATED && in_weights ? in_weights[pair] : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = GATED ? activated(acc[0][e] * wgt, acc[TT - 1][e] * wgt, gate) : acc[0][e];
+      const int n = block * 16 + 4 * q;
+      float* to = out + (size_t)pair * w.rows + n;
+      if (w.rows % 4 == 0) {
+        if (n < w.rows) store_four(to, v[0], v[1], v[2], v[3]);
       } else {
-        out[(size_t)pair * w.rows + n] = sum[0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < w.rows) to[e] = v[e];
       }
     }
   }
+}
+
+// The second product of very few rows, with the sum over a row's pairs: a workgroup owns 8 outputs of a row, its eight waves take the row's
+// pairs in turn, each with half a block of its expert's matrix.  An expert that several rows share is read for each of them.
+// grid (ceil(D / 8), rows).  in float32 [rows * top][K].
+template <typename T, typename TC, bool FULL, int LOAD>
+__global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_sum_kernel(const float* __restrict__ in, const int32_t* __restrict__ chosen,
+                                                                        const float* __restrict__ weights, const T* __restrict__ through, int E, F8Weight w,
+                                                                        TC* __restrict__ out, int K, int top, int fresh) {
+  constexpr int DEPTH = 4;
+  __shared__ __attribute__((aligned(16))) float shares[FEW_TOP][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, i = lane % 16, q = lane / 16;
+  const int row = blockIdx.y, D = w.rows, first = blockIdx.x * 8, block = first / 16, stretches = w.stretches;
+  for (int j = wave; j < top; j += FEW_WAVES) {
+    const long pair = (long)row * top + j;
+    const int expert = chosen[pair];
+    if (expert < 0 || expert >= E) continue;      // the wave
+    const uint8_t* wp = w.data + ((size_t)expert * w.blocks() + block) * stretches * F8_BLOCK + (q * 16 + first % 16 + i % 8) * 16;      // (each of its rows twice)
+    const float* ws = w.scales + ((size_t)expert * w.scale_rows() + block / 8) * stretches;
+    const float* from = in + pair * K;
+    f8_f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    f8_u32x4_t wv[DEPTH][2];
+    float wsv[DEPTH];
+    F8Stretch<float> xv[DEPTH];
+    auto ask = [&](int u, int s) {
+      f8_load_stretch<float, LOAD>(xv[u], from, true, s * F8_K + 16 * q, K);
+      const f8_u32x4_t* at = reinterpret_cast<const f8_u32x4_t*>(wp + (size_t)s * F8_BLOCK);
+      wv[u][0] = at[0], wv[u][1] = at[64];
+      wsv[u] = ws[s];
+    };
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (u < stretches) ask(u, u);
+    for (int n = 0; n < stretches; n += DEPTH)
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u)
+        if (n + u < stretches) {
+          F8Operand<FULL> xo, wo;
+          float xs;
+          xo.set(xv[u].quantised(&xs));
+          wo.set(f8_operand(wv[u][0], wv[u][1]));
+          const f8_f32x4_t sum = f8_stretch(wo, xo);
+          const float s = xs * wsv[u];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(sum[e], s, acc[e]);
+          if (n + u + DEPTH < stretches) ask(u, n + u + DEPTH);
+        }
+    if (i == 0) *reinterpret_cast<f8_f32x4_t*>(&shares[j][4 * q]) = acc;
+  }
+  __syncthreads();
+  const int d = first + threadIdx.x;
+  if (threadIdx.x >= 8 || d >= D) return;
+  float total = 0.f;
+  for (int j = 0; j < top; ++j) {
+    const long pair = (long)row * top + j;
+    const int e = chosen[pair];
+    if (e < 0 || (e >= E && through == nullptr)) continue;
+    total = fmaf(weights ? weights[pair] : 1.0f, e >= E ? to_f32(through[(size_t)row * D + d]) : shares[j][threadIdx.x], total);
+  }
+  TC* at = out + (size_t)row * D + d;
+  *at = from_f32<TC>(fresh ? total : to_f32(*at) + total);
+}
+
+// How many waves share a block: enough workgroups for every compute unit to have one, whatever the pairs.
+int few_shares(int pairs, int E, int N, int stretches) {
+  const long blocks = (long)((N + 15) / 16) * (pairs < E ? pairs : E);      // if no expert is chosen twice
+  int shares = 1;
+  while (shares < 8 && 2 * shares <= stretches && blocks * shares / 8 < 2L * bh_compute_units()) shares *= 2;
+  return shares;
+}
+
+template <typename T, bool GATED, bool FULL, int LOAD>
+void launch_few(const T* in, int in_div, const int32_t* chosen, int pairs, int E, const F8Weight& w, float* out, int K, const ExpertGate& gate,
+                const float* in_weights, hipStream_t stream) {
+  const int shares = few_shares(pairs, E, w.rows, w.stretches), segment = w.stretches < SEGMENT ? w.stretches : SEGMENT;
+  const dim3 grid((w.blocks() * shares + 7) / 8, pairs < E ? pairs : E);
+  const size_t lds = (size_t)segment * (F8_BLOCK + 64);
+#define BH_F8_EXPERTS(KS)                                                                                                                   \
+  do {                                                                                                                                      \
+    bh_allow_lds<experts_few_kernel<T, GATED, FULL, LOAD, KS, (GATED ? 3 : 4)>>(lds);                                                       \
+    experts_few_kernel<T, GATED, FULL, LOAD, KS, (GATED ? 3 : 4)><<<grid, FEW_WAVES * 64, lds, stream>>>(in, in_div, chosen, pairs, E, w, out, K, \
+                                                                                                        gate, in_weights);                  \
+  } while (0)
+  switch (shares) {
+    case 1: BH_F8_EXPERTS(1); break;
+    case 2: BH_F8_EXPERTS(2); break;
+    case 4: BH_F8_EXPERTS(4); break;
+    default: BH_F8_EXPERTS(8);
+  }
+#undef BH_F8_EXPERTS
 }
 
 // ---- tiles -----------------------------------------------------------------------------------------------------
@@ -301,14 +437,12 @@ extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, con
   BH_REQUIRE(pairs > 0 && pairs <= FEW_PAIRS && E > 0 && N > 0 && K > 0 && in_div > 0, "experts_float8: 1 to %d pairs of positive sizes, got %d", FEW_PAIRS, pairs);
   BH_REQUIRE((uintptr_t)w % 16 == 0, "experts_float8: the weights must be 16-byte aligned");
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
-  const dim3 grid(weight.blocks(), pairs < E ? pairs : E);
-  BH_REQUIRE(grid.y <= 65535, "experts_float8: up to 65,535 experts");
-  const int load = f8_load_of(in, K);
+  BH_REQUIRE(E <= 65535, "experts_float8: up to 65,535 experts, got %d", E);
   const ExpertGate gate = {limit, alpha, shift};
-#define BH_F8_EXPERTS(T, GATED, FULL)                                                                                                                   \
-  do {                                                                                                                                                  \
-    if (load == F8_EVEN) experts_few_kernel<T, GATED, FULL, F8_EVEN><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights); \
-    else experts_few_kernel<T, GATED, FULL, F8_VALUES><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights);      \
+#define BH_F8_EXPERTS(T, GATED, FULL)                                                                                                              \
+  do {                                                                                                                                             \
+    if (f8_load_of(in, K) == F8_EVEN) launch_few<T, GATED, FULL, F8_EVEN>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights, stream); \
+    else launch_few<T, GATED, FULL, F8_VALUES>((const T*)in, in_div, chosen, pairs, E, weight, out, K, gate, in_weights, stream);                  \
   } while (0)
 #define BH_F8_EXPERTS_OF(T)                                                                                \
   do {                                                                                                     \
@@ -318,7 +452,41 @@ extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, con
   if (dtype == BH_F32) BH_F8_EXPERTS_OF(float);
   else if (dtype == BH_BF16) BH_F8_EXPERTS_OF(bf16_t);
   else return bh_fail("experts_float8: unknown dtype %d", dtype);
+#undef BH_F8_EXPERTS_OF
+#undef BH_F8_EXPERTS
   return bh_check_launch("experts_float8_rows");
+}
+
+// Whether the second product of `few` sums a row's pairs itself: rows of so few pairs that an expert is hardly chosen twice.
+extern "C" int bh_experts_float8_sums(int pairs, int E, int top) { return pairs <= FEW_PAIRS && top <= FEW_TOP && 4 * pairs <= E; }
+
+// That product: in float32 [n_rows * top][K], out [n_rows][D].
+extern "C" int bh_experts_float8_rows_sum(const float* in, const int32_t* chosen, const float* weights, const void* through, int dtype, const void* w,
+                                          const void* scales, void* out, int c_dtype, int n_rows, int E, int top, int D, int K, int fresh, int full,
+                                          hipStream_t stream) {
+  BH_REQUIRE(n_rows > 0 && n_rows <= 65535 && top > 0 && top <= FEW_TOP && D > 0 && K > 0 && E > 0, "experts_float8: %d rows of %d pairs of %d outputs", n_rows, top, D);
+  BH_REQUIRE((uintptr_t)w % 16 == 0, "experts_float8: the weights must be 16-byte aligned");
+  BH_REQUIRE((dtype == BH_F32 || dtype == BH_BF16) && (c_dtype == BH_F32 || c_dtype == BH_BF16), "experts_float8: unknown dtype");
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, D, (K + F8_K - 1) / F8_K};
+  const dim3 grid((D + 7) / 8, n_rows);
+#define BH_F8_SUM_AS(T, TC, FULL, LOAD) \
+  experts_few_sum_kernel<T, TC, FULL, LOAD><<<grid, FEW_WAVES * 64, 0, stream>>>(in, chosen, weights, (const T*)through, E, weight, (TC*)out, K, top, fresh)
+#define BH_F8_SUM(T, TC)                                                      \
+  do {                                                                        \
+    if (f8_load_of(in, K) == F8_EVEN) {                                       \
+      if (full) BH_F8_SUM_AS(T, TC, true, F8_EVEN);                           \
+      else BH_F8_SUM_AS(T, TC, false, F8_EVEN);                               \
+    } else if (full) BH_F8_SUM_AS(T, TC, true, F8_VALUES);                    \
+    else BH_F8_SUM_AS(T, TC, false, F8_VALUES);                               \
+  } while (0)
+  if (dtype == BH_F32) {
+    if (c_dtype == BH_F32) BH_F8_SUM(float, float);
+    else BH_F8_SUM(float, bf16_t);
+  } else if (c_dtype == BH_F32) BH_F8_SUM(bf16_t, float);
+  else BH_F8_SUM(bf16_t, bf16_t);
+#undef BH_F8_SUM
+#undef BH_F8_SUM_AS
+  return bh_check_launch("experts_float8_rows_sum");
 }
 
 // One of the two products of `tiles`, from rows in 8 bits; lists [E][capacity] and counts [E] as experts_group makes them.  Gated: out is

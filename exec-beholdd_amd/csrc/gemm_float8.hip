@@ -286,8 +286,8 @@ int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int 
 
 }  // namespace
 
-// Whether a product of M rows takes them as they are (`few`); otherwise they are brought into 8 bits first.
-extern "C" int bh_gemm_float8_takes_rows(int M) { return M <= FEW_ROWS; }
+// Up to so many rows a product takes them as they are (`few`); more are brought into 8 bits first.
+extern "C" int bh_gemm_float8_few_rows() { return FEW_ROWS; }
 // Bytes of scratch memory of a product from rows in 8 bits.
 extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full) {
   if (M <= FEW_ROWS_IN_8 || N <= 0 || K <= 0 || float8_ring_tile(M, N, K, gated != 0, full != 0) >= 0) return 0;

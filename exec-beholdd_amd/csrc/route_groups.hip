@@ -7,6 +7,10 @@
 // A row is a wave's.  Choices are whole numbers that a rounding would change, and scores of two experts differ by less than 32 bits tell
 // apart in one row of 30,000 (256 experts): scores, merits and sums are in 64 bits, whose exponentials are a small part of the time.
 // A score that is not a number counts as the lowest, so that the indices are always `top` different experts of open groups.
+// Bound by the chain of `top` choices for few rows, by their instructions for many.  A choice finds the largest upper half of the scores' bits,
+// ordered as whole numbers, in six steps between registers of neighbouring lanes; only where two lanes share it (one choice in thousands, or equal
+// scores) the lower halves and the indices are compared.  Measured, us, in brackets with 64-bit scores, indices and weights handed between lanes
+// through LDS at every step: 1 row of 128 4.7 (8.8), 1,234 of 160 8.4 (11.7), 8,192 of 256 20.1 (31.7).
 #include "common.h"
 
 #define RG_MAX_TOP 32
@@ -21,6 +25,32 @@ struct Two {
 __device__ inline Two merged(Two a, Two b) {
   const bool mine = a.first >= b.first;
   return {mine ? a.first : b.first, mine ? fmax(a.second, b.first) : fmax(b.second, a.first)};
+}
+
+// The largest (or smallest) over the wave, for every lane.
+template <typename JOIN>
+__device__ inline uint32_t over_wave(uint32_t v, JOIN join) {
+  v = join(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128 /* row_ror:8 */, 0xf, 0xf, true));
+  v = join(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+  v = join(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+  v = join(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = join((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return join((uint32_t)b[0], (uint32_t)b[1]);
+}
+__device__ inline uint32_t wave_largest(uint32_t v) {
+  return over_wave(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+// A number's bits in the order of the numbers; above 0, which stands for none.
+__device__ inline unsigned long long ordered(double v) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  return bits >> 63 ? ~bits : bits | (1ull << 63);
+}
+__device__ inline double of_lane(double v, int lane) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t low = __builtin_amdgcn_readlane((int)bits, lane), high = __builtin_amdgcn_readlane((int)(bits >> 32), lane);
+  return __builtin_bit_cast(double, (unsigned long long)high << 32 | low);
 }
 
 __device__ inline double wave_sum_f64(double v) {
@@ -68,7 +98,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
   for (int i = 0; i < PER; ++i) {
     const int e = lane + i * BH_WAVE;
     by[i] = e < E ? score[i] + (correction ? (double)correction[e] : 0.) : none;
-    if (!(by[i] == by[i])) by[i] = none;
+    by[i] = by[i] == by[i] ? by[i] + 0. : none;      // (a negative zero becomes a positive one, whose bits it then shares)
   }
   unsigned taken = 0;      // bit i: this lane's expert lane + 64 i may not be chosen (any more)
 #pragma unroll
@@ -103,31 +133,41 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
   }
   double sum = 0., mine = 0.;      // lane j keeps the j-th choice
   int mine_index = 0;
-  for (int j = 0; j < top; ++j) {
-    double best = none, best_score = 0.;
-    int best_e = 0x7fffffff;
+  unsigned long long best = 0;      // of this lane's experts that may be chosen, with its score
+  double best_score = 0.;
+  int best_e = 0;
+  auto find_best = [&]() {
+    best = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (!((taken >> i) & 1u) && (by[i] > best || best_e == 0x7fffffff)) {
-        best = by[i];
+    for (int i = 0; i < PER; ++i) {
+      const unsigned long long key = (taken >> i) & 1u ? 0 : ordered(by[i]);
+      if (key > best) {
+        best = key;
         best_score = score[i];
         best_e = lane + i * BH_WAVE;
       }
-#pragma unroll
-    for (int off = BH_WAVE / 2; off > 0; off >>= 1) {
-      const double other = __shfl_xor(best, off, BH_WAVE), other_score = __shfl_xor(best_score, off, BH_WAVE);
-      const int other_e = __shfl_xor(best_e, off, BH_WAVE);
-      if (other_e != 0x7fffffff && (best_e == 0x7fffffff || other > best || (other == best && other_e < best_e))) {
-        best = other;
-        best_score = other_score;
-        best_e = other_e;
-      }
     }
-    if (best_e % BH_WAVE == lane) taken |= 1u << (best_e / BH_WAVE);
-    sum += best_score;
+  };
+  find_best();
+  for (int j = 0; j < top; ++j) {
+    const uint32_t high = (uint32_t)(best >> 32), most = wave_largest(high);
+    unsigned long long having = __ballot(high == most);
+    if (having & (having - 1)) {      // several lanes: the lower halves decide, then the index
+      const uint32_t low = high == most ? (uint32_t)best : 0u, most_low = wave_largest(low);
+      const uint32_t index = high == most && low == most_low ? (uint32_t)best_e : 0xffffffffu;
+      having = __ballot(index == over_wave(index, [](uint32_t a, uint32_t b) { return min(a, b); }) && high == most);
+    }
+    const int winner = __builtin_amdgcn_readfirstlane(__ffsll(having) - 1);
+    const int e = __builtin_amdgcn_readlane(best_e, winner);
+    const double p = of_lane(best_score, winner);
+    sum += p;
     if (lane == j) {
-      mine = best_score;
-      mine_index = best_e;
+      mine = p;
+      mine_index = e;
+    }
+    if (lane == winner) {
+      taken |= 1u << (e / BH_WAVE);
+      find_best();
     }
   }
   if (lane < top) {

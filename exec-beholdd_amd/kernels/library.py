@@ -300,12 +300,14 @@ class KernelSizes:
             "bh_weighted_sum": [p, p, f, p, f, ctypes.c_long, p],
             "bh_experts_combine": [p, p, p, p, p, i, p, i, i, i, i, i, p],
             "bh_float8_rows": [p, i, p, p, i, i, i, i, p],
-            "bh_gemm_float8_takes_rows": [i],
+            "bh_gemm_float8_few_rows": [],
             "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
             "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
             "bh_experts_float8_few": [i, i],
             "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
+            "bh_experts_float8_sums": [i, i, i],
+            "bh_experts_float8_rows_sum": [p, p, p, p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, p, i, i, i, f, f, f, p, i, p],
             "bh_experts_float8_sum": [p, p, p, p, i, p, i, i, i, i, i, i, p],
         }
@@ -442,6 +444,9 @@ class HipKernels(KernelSizes):
         self._squares: dict = {}    # (m, n, k) -> which product squares its output (`gemm_relu_squared`), or 0
         self._clamps: dict = {}     # (m, n, k) -> which gated product clamps (`gemm_clamped_glu`), or 0
         self._bare: dict = {}       # (m, n, k) -> the parts that `gemm_bare` leaves such a product in, or 0
+        self._float8_scratch: dict = {}      # (m, n, k, gated, full sums) -> scratch bytes of a product from rows in 8 bits
+        self._float8_experts: dict = {}      # (pairs, experts, top) -> whether few pairs' kernels take them, and whether the second sums them
+        self._float8_few_rows = int(self.lib.bh_gemm_float8_few_rows())      # up to so many rows a product takes them as they are
         self.page_size = int(self.lib.bh_page_size())
         if self.page_size != _build.source_page_size():
             raise KernelError(f"{self.library_path} was built for pages of {self.page_size} tokens, the sources say "
@@ -968,29 +973,38 @@ class HipKernels(KernelSizes):
     def _gemm_float8(self, a, w, out, accumulate, gate, full_sums):
         """out (+)= a times a `Float8Weight`, plain (gate 0) or gated."""
         (m, k), n, matrices = a.shape, w.rows, 1 if gate else w.matrices
-        full = out.dtype == torch.float32 if full_sums is None else bool(full_sums)
+        full = int(out.dtype == torch.float32 if full_sums is None else bool(full_sums))
         if isinstance(out, BlockedRows):
             raise KernelError("gemm: a product with an 8-bit weight writes plain rows")
-        if isinstance(a, Float8Rows):
-            if a.in_rows:
-                raise KernelError("gemm: rows in 8 bits go into a product in blocks")
-        else:
-            a = self._plain_rows(a)
-            if not self.lib.bh_gemm_float8_takes_rows(m):
-                self._ptr(a, "gemm a", tuple(_CODES))
-                a = self.to_float8(a)
-        out_at, c_code, stream = self._ptr(out, "gemm out"), _code(out, "gemm out"), self._stream()
-        for i in range(matrices):
-            data = w.data.data_ptr() + i * Float8Weight.data_bytes(1, n, k)
-            scales, at = w.scales.data_ptr() + i * w.scales[0].numel() * 4, out_at + i * n * out.element_size()
+        few = type(a) is torch.Tensor and m <= self._float8_few_rows
+        if not few:
             if not isinstance(a, Float8Rows):
-                self._check(self.lib.bh_gemm_float8_few(self._ptr(a, "gemm a"), _code(a, "gemm a"), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
-                                                        out.shape[1], gate, int(full), stream))
-                continue
-            scratch_bytes = int(self.lib.bh_gemm_float8_scratch(m, n, k, int(gate != 0), int(full)))
+                a = self._plain_rows(a)
+                few = m <= self._float8_few_rows
+                if not few:
+                    a = self.to_float8(a)
+            elif a.in_rows:
+                raise KernelError("gemm: rows in 8 bits go into a product in blocks")
+        out_at, c_code, stream, accumulate = self._ptr(out, "gemm out"), _code(out, "gemm out"), self._stream(), int(bool(accumulate))
+        data, scales = w.data.data_ptr(), w.scales.data_ptr()
+        if few:
+            a_at, a_code = self._ptr(a, "gemm a"), _code(a, "gemm a")
+        else:
+            key = (m, n, k, gate != 0, full)
+            scratch_bytes = self._float8_scratch.get(key)
+            if scratch_bytes is None:
+                scratch_bytes = self._float8_scratch[key] = int(self.lib.bh_gemm_float8_scratch(*map(int, key)))
             scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=self.device) if scratch_bytes else None
-            self._check(self.lib.bh_gemm_float8(a.data.data_ptr(), a.exponents.data_ptr(), data, scales, at, c_code, int(bool(accumulate)), m, n, k,
-                                                out.shape[1], gate, int(full), scratch.data_ptr() if scratch is not None else None, stream))
+            a_at, exponents, scratch_at = a.data.data_ptr(), a.exponents.data_ptr(), scratch.data_ptr() if scratch is not None else None
+        for i in range(matrices):
+            if i:
+                data, out_at = data + Float8Weight.data_bytes(1, n, k), out_at + n * out.element_size()
+                scales += 4 * w.scales.shape[1] * w.scales.shape[2]
+            if few:
+                self._check(self.lib.bh_gemm_float8_few(a_at, a_code, data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1], gate, full, stream))
+            else:
+                self._check(self.lib.bh_gemm_float8(a_at, exponents, data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1], gate, full, scratch_at,
+                                                    stream))
 
     def experts_float8(self, x, chosen, weights, w_up, w_down, out, limit=float("inf"), alpha=1.0, shift=0.0, weigh_input=False, fresh=False, through=None,
                        full_sums=None):
@@ -1018,12 +1032,21 @@ class HipKernels(KernelSizes):
         act = (float(limit), float(alpha), float(shift))
         x_at, x_code, out_at, out_code = self._ptr(x, "experts x"), _code(x, "experts x"), self._ptr(out, "experts out"), _code(out, "experts out")
         through_at = self._ptr(through, "experts input", None, True)
-        y = torch.empty((pairs, width), dtype=torch.float32, device=self.device)
-        in_weights = weights_at if weigh_input else None
-        if lib.bh_experts_float8_few(pairs, experts):
+        in_weights, out_weights = (weights_at, None) if weigh_input else (None, weights_at)
+        plan = self._float8_experts.get((pairs, experts, top))
+        if plan is None:
+            plan = self._float8_experts[(pairs, experts, top)] = (bool(lib.bh_experts_float8_few(pairs, experts)), bool(lib.bh_experts_float8_sums(pairs, experts, top)))
+        few, sums = plan
+        y = None if sums else torch.empty((pairs, width), dtype=torch.float32, device=self.device)
+        if few:
             inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
             self._check(lib.bh_experts_float8_rows(x_at, x_code, top, chosen_at, pairs, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(),
                                                    ff, k, 1, *act, in_weights, int(full_up), stream))
+            if sums:
+                self._check(lib.bh_experts_float8_rows_sum(inner.data_ptr(), chosen_at, out_weights, through_at, x_code, w_down.data.data_ptr(),
+                                                           w_down.scales.data_ptr(), out_at, out_code, n, experts, top, width, ff, int(bool(fresh)), int(full),
+                                                           stream))
+                return
             self._check(lib.bh_experts_float8_rows(inner.data_ptr(), F32, 1, chosen_at, pairs, experts, w_down.data.data_ptr(), w_down.scales.data_ptr(),
                                                    y.data_ptr(), width, ff, 0, *act, None, int(full), stream))
         else:
@@ -1038,7 +1061,7 @@ class HipKernels(KernelSizes):
                     a.data.data_ptr(), a.exponents.data_ptr(), in_rows, div, lists.data_ptr(), pairs, counts.data_ptr(), pairs, experts, w.data.data_ptr(),
                     w.scales.data_ptr(), out_rows.data_ptr(), out_exponents.data_ptr() if gated else None, outs, ins, int(gated), *act,
                     in_weights if gated else None, int(is_full), stream))
-        self._check(lib.bh_experts_float8_sum(y.data_ptr(), chosen_at, None if weigh_input else weights_at, through_at, x_code, out_at, out_code, n, experts, top,
+        self._check(lib.bh_experts_float8_sum(y.data_ptr(), chosen_at, out_weights, through_at, x_code, out_at, out_code, n, experts, top,
                                               width, int(bool(fresh)), stream))
 
     def qk_norm_rope_cache(self, qkv, q_out, q_weight, k_weight, eps, cos, sin, positions, row_seq,

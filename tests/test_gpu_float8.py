@@ -245,7 +245,7 @@ def _experts(k, n, width, ff, e, top, dtype, seed, out_of_range=False):
     return _rows(n, width, dtype, seed), chosen, weights, (up, down), (held_up, held_down)
 
 
-EXPERTS = [(1, 128, 128, 4, 2), (1, 130, 33, 1, 1), (3, 64, 48, 8, 3), (20, 300, 129, 3, 4), (70, 257, 144, 2, 2), (150, 128, 64, 5, 4), (64, 96, 20, 70, 1)]
+EXPERTS = [(1, 128, 128, 4, 2), (1, 130, 33, 1, 1), (3, 64, 48, 8, 3), (20, 300, 129, 3, 4), (70, 257, 144, 2, 2), (150, 128, 64, 5, 4), (64, 96, 20, 70, 1), (2, 144, 100, 40, 5), (1, 256, 130, 64, 16), (1, 20, 4200, 9, 2), (4, 4300, 16, 6, 3)]
 
 
 @pytest.mark.parametrize("n,width,ff,e,top", EXPERTS)
@@ -263,7 +263,7 @@ def test_experts(k, n, width, ff, e, top, dtype, out_dtype):
     _close(fresh, want, bound)
 
 
-@pytest.mark.parametrize("n,e", [(4, 6), (90, 3)])
+@pytest.mark.parametrize("n,e", [(1, 12), (4, 6), (90, 3)])
 @pytest.mark.parametrize("form", ["through", "none_of_them", "weigh_input", "clamped"])
 def test_forms_of_experts(k, n, e, form):
     x, chosen, weights, packed, held = _experts(k, n, 200, 136, e, 3, torch.bfloat16, 31, out_of_range=form in ("through", "none_of_them"))
