@@ -4,7 +4,8 @@
 //   out[row] (+)= sum over j of weight[p] * y[p], j in order
 // A pair's weight may multiply the expert's input instead (its gate and up sums).  A pair whose expert is none of the E gives nothing, or,
 // with `through`, one numbered E or higher hands the row's input on.  Nothing here depends on the routing on the host.
-//   few    an expert's pairs 16 at a time, quantised by the waves that multiply them (gemm_float8.hip's product of few rows)
+//   one    the pairs of one row
+//   few    an expert's pairs 16 at a time, brought into 8 bits by the workgroup that multiplies them
 //   tiles  tiles of 64 or 128 pairs of an expert from rows in 8 bits, found from the experts' counts by every workgroup itself
 #include "float8_few.h"
 #include "float8_ring.h"
@@ -26,7 +27,7 @@ __device__ inline float activated(float g, float u, const ExpertGate& gate) {
 // up to 16 of the expert's pairs are brought into 8 bits once for the workgroup and kept in LDS, F8_SEGMENT stretches of k at a time, while
 // the first weights are on their way.
 constexpr int FEW_WAVES = 8, FEW_PAIRS = 1024;      // pairs of a call at most
-constexpr int FEW_TOP = 32;                         // pairs of a row, where the second product sums them itself
+constexpr int FEW_TOP = 32;                         // pairs of a row alone, at most
 constexpr int SEGMENT = 32;                         // stretches of the rows that LDS holds
 
 // grid (ceil(blocks / (8 / KS)), min(pairs, E)).  With at most E pairs a workgroup is a pair's, and the first pair of an expert does all of
@@ -168,41 +169,123 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_kernel(const T* __
   }
 }
 
-// The second product of very few rows, with the sum over a row's pairs: a workgroup owns 8 outputs of a row, its eight waves take the row's
-// pairs in turn, each with half a block of its expert's matrix.  An expert that several rows share is read for each of them.
-// grid (ceil(D / 8), rows).  in float32 [rows * top][K].
+// ---- one row ---------------------------------------------------------------------------------------------------
+// A step of one row is two trips to memory in a row (the choice, then the matrices) twice over: both products as short as that chain.
+// The first product: a workgroup owns 16 outputs of a pair, its eight waves take the stretches of k in turn and bring the row into 8 bits
+// themselves; the row does not wait for the choice.  grid (ceil(N / 16), top).  (As one of the workgroups of `few`, which look for the pairs of
+// their expert first and keep its rows in LDS, 25 MB took 13.2 us, 8.0 so.)
+template <typename T, bool FULL, int LOAD>
+__global__ __launch_bounds__(FEW_WAVES * 64) void experts_one_kernel(const T* __restrict__ row, const int32_t* __restrict__ chosen, int E, F8Weight w,
+                                                                    float* __restrict__ out, int K, ExpertGate gate, const float* __restrict__ in_weights) {
+  constexpr int DEPTH = 2;
+  __shared__ __attribute__((aligned(16))) float partial[FEW_WAVES][2][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, i = lane % 16, q = lane / 16;
+  const int pair = blockIdx.y, block = blockIdx.x, blocks = w.blocks(), stretches = w.stretches, left = (stretches - wave + FEW_WAVES - 1) / FEW_WAVES;
+  F8Stretch<T> xv[DEPTH];
+  auto ask_row = [&](int u, int n) { f8_load_stretch<T, LOAD>(xv[u], row, true, (wave + n * FEW_WAVES) * F8_K + 16 * q, K); };
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u)
+    if (u < left) ask_row(u, u);
+  const int expert = chosen[pair];
+  if (expert < 0 || expert >= E) return;      // the whole workgroup
+  const float wgt = in_weights ? in_weights[pair] : 1.0f;
+  const uint8_t* wp[2];
+  const float* ws[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const size_t matrix = 2 * (size_t)expert + t;
+    wp[t] = w.data + (matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
+    ws[t] = w.scales + (matrix * w.scale_rows() + block / 8) * stretches;
+  }
+  f8_u32x4_t wv[DEPTH][2][2];
+  float wsv[DEPTH][2];
+  auto ask = [&](int u, int n) {
+    const int j = wave + n * FEW_WAVES;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f8_u32x4_t* from = reinterpret_cast<const f8_u32x4_t*>(wp[t] + (size_t)j * F8_BLOCK);
+      wv[u][t][0] = __builtin_nontemporal_load(from);
+      wv[u][t][1] = __builtin_nontemporal_load(from + 64);
+      wsv[u][t] = ws[t][j];
+    }
+  };
+  f8_f32x4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u)
+    if (u < left) ask(u, u);
+  for (int n = 0; n < left; n += DEPTH)
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (n + u < left) {
+        F8Operand<FULL> xo, wo;
+        float xs;
+        xo.set(xv[u].quantised(&xs));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
+          const f8_f32x4_t sum = f8_stretch(wo, xo);
+          const float s = xs * wsv[u][t];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sum[e], s, acc[t][e]);
+        }
+        if (n + u + DEPTH < left) ask_row(u, n + u + DEPTH), ask(u, n + u + DEPTH);
+      }
+  if (i == 0) {      // (all rows of the operand are the row)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) *reinterpret_cast<f8_f32x4_t*>(&partial[wave][t][4 * q]) = acc[t];
+  }
+  __syncthreads();
+  const int n = block * 16 + threadIdx.x;
+  if (threadIdx.x >= 16 || n >= w.rows) return;
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < FEW_WAVES; ++v)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sum[t] += partial[v][t][threadIdx.x];
+  out[(size_t)pair * w.rows + n] = activated(sum[0] * wgt, sum[1] * wgt, gate);
+}
+
+// The second product with the sum over the pairs: a workgroup owns 8 outputs, its sixteen waves share the pairs out between them, several
+// waves a pair where there are few, each with half a block of its expert's matrix.  grid (ceil(D / 8)).  in float32 [top][K].
+constexpr int ONE_WAVES = 16;
 template <typename T, typename TC, bool FULL, int LOAD>
-__global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_sum_kernel(const float* __restrict__ in, const int32_t* __restrict__ chosen,
+__global__ __launch_bounds__(ONE_WAVES * 64) void experts_one_sum_kernel(const float* __restrict__ in, const int32_t* __restrict__ chosen,
                                                                         const float* __restrict__ weights, const T* __restrict__ through, int E, F8Weight w,
                                                                         TC* __restrict__ out, int K, int top, int fresh) {
-  constexpr int DEPTH = 4;
-  __shared__ __attribute__((aligned(16))) float shares[FEW_TOP][16];
+  constexpr int DEPTH = 2;
+  __shared__ __attribute__((aligned(16))) float shares[FEW_TOP][ONE_WAVES][8];      // [pair][wave of the pair][output]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, i = lane % 16, q = lane / 16;
-  const int row = blockIdx.y, D = w.rows, first = blockIdx.x * 8, block = first / 16, stretches = w.stretches;
-  for (int j = wave; j < top; j += FEW_WAVES) {
-    const long pair = (long)row * top + j;
-    const int expert = chosen[pair];
+  const int D = w.rows, first = blockIdx.x * 8, block = first / 16, stretches = w.stretches;
+  const int split = top >= ONE_WAVES ? 1 : ONE_WAVES / top, part = wave % split, at_once = ONE_WAVES / split;      // waves of a pair; pairs at a time
+  const int left = (stretches - part + split - 1) / split;
+  for (int j = wave / split; j < top && wave < split * at_once; j += at_once) {
+    const float* from = in + (size_t)j * K;
+    F8Stretch<float> xv[DEPTH];
+    auto ask_row = [&](int u, int n) { f8_load_stretch<float, LOAD>(xv[u], from, true, (part + n * split) * F8_K + 16 * q, K); };
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (u < left) ask_row(u, u);
+    const int expert = chosen[j];
     if (expert < 0 || expert >= E) continue;      // the wave
     const uint8_t* wp = w.data + ((size_t)expert * w.blocks() + block) * stretches * F8_BLOCK + (q * 16 + first % 16 + i % 8) * 16;      // (each of its rows twice)
     const float* ws = w.scales + ((size_t)expert * w.scale_rows() + block / 8) * stretches;
-    const float* from = in + pair * K;
     f8_f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     f8_u32x4_t wv[DEPTH][2];
     float wsv[DEPTH];
-    F8Stretch<float> xv[DEPTH];
-    auto ask = [&](int u, int s) {
-      f8_load_stretch<float, LOAD>(xv[u], from, true, s * F8_K + 16 * q, K);
+    auto ask = [&](int u, int n) {
+      const int s = part + n * split;
       const f8_u32x4_t* at = reinterpret_cast<const f8_u32x4_t*>(wp + (size_t)s * F8_BLOCK);
-      wv[u][0] = at[0], wv[u][1] = at[64];
+      wv[u][0] = __builtin_nontemporal_load(at);
+      wv[u][1] = __builtin_nontemporal_load(at + 64);
       wsv[u] = ws[s];
     };
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u)
-      if (u < stretches) ask(u, u);
-    for (int n = 0; n < stretches; n += DEPTH)
+      if (u < left) ask(u, u);
+    for (int n = 0; n < left; n += DEPTH)
 #pragma unroll
       for (int u = 0; u < DEPTH; ++u)
-        if (n + u < stretches) {
+        if (n + u < left) {
           F8Operand<FULL> xo, wo;
           float xs;
           xo.set(xv[u].quantised(&xs));
@@ -211,22 +294,29 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void experts_few_sum_kernel(const f
           const float s = xs * wsv[u];
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[e] = fmaf(sum[e], s, acc[e]);
-          if (n + u + DEPTH < stretches) ask(u, n + u + DEPTH);
+          if (n + u + DEPTH < left) ask_row(u, n + u + DEPTH), ask(u, n + u + DEPTH);
         }
-    if (i == 0) *reinterpret_cast<f8_f32x4_t*>(&shares[j][4 * q]) = acc;
+    if (i == 0 && q < 2) *reinterpret_cast<f8_f32x4_t*>(&shares[j][part][4 * q]) = acc;
   }
+  // lane j of the first wave knows pair j's expert and weight before the shares are there
+  const int own = chosen[min(lane, top - 1)];
+  const float own_weight = weights ? weights[min(lane, top - 1)] : 1.0f;
   __syncthreads();
-  const int d = first + threadIdx.x;
-  if (threadIdx.x >= 8 || d >= D) return;
+  if (wave) return;
+  const int d = first + lane;
   float total = 0.f;
   for (int j = 0; j < top; ++j) {
-    const long pair = (long)row * top + j;
-    const int e = chosen[pair];
-    if (e < 0 || (e >= E && through == nullptr)) continue;
-    total = fmaf(weights ? weights[pair] : 1.0f, e >= E ? to_f32(through[(size_t)row * D + d]) : shares[j][threadIdx.x], total);
+    const int e = __builtin_amdgcn_readlane(own, j);
+    const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own_weight), j));
+    if (e < 0 || (e >= E && through == nullptr) || lane >= 8 || d >= D) continue;
+    float y = 0.f;
+    if (e >= E) y = to_f32(through[d]);
+    else
+      for (int v = 0; v < split; ++v) y += shares[j][v][lane];
+    total = fmaf(f, y, total);
   }
-  TC* at = out + (size_t)row * D + d;
-  *at = from_f32<TC>(fresh ? total : to_f32(*at) + total);
+  if (lane >= 8 || d >= D) return;
+  out[d] = from_f32<TC>(fresh ? total : to_f32(out[d]) + total);
 }
 
 // How many waves share a block: enough workgroups for every compute unit to have one, whatever the pairs.
@@ -457,23 +547,41 @@ extern "C" int bh_experts_float8_rows(const void* in, int dtype, int in_div, con
   return bh_check_launch("experts_float8_rows");
 }
 
-// Whether the second product of `few` sums a row's pairs itself: rows of so few pairs that an expert is hardly chosen twice.
-extern "C" int bh_experts_float8_sums(int pairs, int E, int top) { return pairs <= FEW_PAIRS && top <= FEW_TOP && 4 * pairs <= E; }
+// Whether a call is one row's.
+extern "C" int bh_experts_float8_one(int pairs, int top) { return pairs == top && top <= FEW_TOP; }
 
-// That product: in float32 [n_rows * top][K], out [n_rows][D].
-extern "C" int bh_experts_float8_rows_sum(const float* in, const int32_t* chosen, const float* weights, const void* through, int dtype, const void* w,
-                                          const void* scales, void* out, int c_dtype, int n_rows, int E, int top, int D, int K, int fresh, int full,
-                                          hipStream_t stream) {
-  BH_REQUIRE(n_rows > 0 && n_rows <= 65535 && top > 0 && top <= FEW_TOP && D > 0 && K > 0 && E > 0, "experts_float8: %d rows of %d pairs of %d outputs", n_rows, top, D);
-  BH_REQUIRE((uintptr_t)w % 16 == 0, "experts_float8: the weights must be 16-byte aligned");
+// Both products of one row and the sum: inner float32 [top][ff] is scratch.
+extern "C" int bh_experts_float8_row(const void* x, int dtype, const int32_t* chosen, const float* weights, int weigh_input, const void* through, int E,
+                                     const void* up, const void* up_scales, const void* down, const void* down_scales, float* inner, void* out, int c_dtype,
+                                     int top, int K, int ff, int D, float limit, float alpha, float shift, int fresh, int full_up, int full, hipStream_t stream) {
+  BH_REQUIRE(top > 0 && top <= FEW_TOP && D > 0 && K > 0 && ff > 0 && E > 0, "experts_float8: a row of %d pairs, %d x %d x %d", top, K, ff, D);
+  BH_REQUIRE(((uintptr_t)up | (uintptr_t)down) % 16 == 0, "experts_float8: the weights must be 16-byte aligned");
   BH_REQUIRE((dtype == BH_F32 || dtype == BH_BF16) && (c_dtype == BH_F32 || c_dtype == BH_BF16), "experts_float8: unknown dtype");
-  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, D, (K + F8_K - 1) / F8_K};
-  const dim3 grid((D + 7) / 8, n_rows);
+  BH_REQUIRE(!weigh_input || weights != nullptr, "experts_float8: inputs are weighed by weights");
+  const F8Weight first = {(const uint8_t*)up, (const float*)up_scales, ff, (K + F8_K - 1) / F8_K};
+  const F8Weight second = {(const uint8_t*)down, (const float*)down_scales, D, (ff + F8_K - 1) / F8_K};
+  const ExpertGate gate = {limit, alpha, shift};
+  const float* in_weights = weigh_input ? weights : nullptr;
+  const float* out_weights = weigh_input ? nullptr : weights;
+#define BH_F8_ONE_AS(T, FULL, LOAD) \
+  experts_one_kernel<T, FULL, LOAD><<<dim3(first.blocks(), top), FEW_WAVES * 64, 0, stream>>>((const T*)x, chosen, E, first, inner, K, gate, in_weights)
+#define BH_F8_ONE(T)                                         \
+  do {                                                       \
+    if (f8_load_of(x, K) == F8_EVEN) {                       \
+      if (full_up) BH_F8_ONE_AS(T, true, F8_EVEN);           \
+      else BH_F8_ONE_AS(T, false, F8_EVEN);                  \
+    } else if (full_up) BH_F8_ONE_AS(T, true, F8_VALUES);    \
+    else BH_F8_ONE_AS(T, false, F8_VALUES);                  \
+  } while (0)
+  if (dtype == BH_F32) BH_F8_ONE(float);
+  else BH_F8_ONE(bf16_t);
+#undef BH_F8_ONE
+#undef BH_F8_ONE_AS
 #define BH_F8_SUM_AS(T, TC, FULL, LOAD) \
-  experts_few_sum_kernel<T, TC, FULL, LOAD><<<grid, FEW_WAVES * 64, 0, stream>>>(in, chosen, weights, (const T*)through, E, weight, (TC*)out, K, top, fresh)
+  experts_one_sum_kernel<T, TC, FULL, LOAD><<<(D + 7) / 8, ONE_WAVES * 64, 0, stream>>>(inner, chosen, out_weights, (const T*)through, E, second, (TC*)out, ff, top, fresh)
 #define BH_F8_SUM(T, TC)                                                      \
   do {                                                                        \
-    if (f8_load_of(in, K) == F8_EVEN) {                                       \
+    if (f8_load_of(inner, ff) == F8_EVEN) {                                   \
       if (full) BH_F8_SUM_AS(T, TC, true, F8_EVEN);                           \
       else BH_F8_SUM_AS(T, TC, false, F8_EVEN);                               \
     } else if (full) BH_F8_SUM_AS(T, TC, true, F8_VALUES);                    \
@@ -486,7 +594,7 @@ extern "C" int bh_experts_float8_rows_sum(const float* in, const int32_t* chosen
   else BH_F8_SUM(bf16_t, bf16_t);
 #undef BH_F8_SUM
 #undef BH_F8_SUM_AS
-  return bh_check_launch("experts_float8_rows_sum");
+  return bh_check_launch("experts_float8_row");
 }
 
 // One of the two products of `tiles`, from rows in 8 bits; lists [E][capacity] and counts [E] as experts_group makes them.  Gated: out is

@@ -306,8 +306,8 @@ class KernelSizes:
             "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
             "bh_experts_float8_few": [i, i],
             "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
-            "bh_experts_float8_sums": [i, i, i],
-            "bh_experts_float8_rows_sum": [p, p, p, p, i, p, p, p, i, i, i, i, i, i, i, i, p],
+            "bh_experts_float8_one": [i, i],
+            "bh_experts_float8_row": [p, i, p, p, i, p, i, p, p, p, p, p, p, i, i, i, i, i, f, f, f, i, i, i, p],
             "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, p, i, i, i, f, f, f, p, i, p],
             "bh_experts_float8_sum": [p, p, p, p, i, p, i, i, i, i, i, i, p],
         }
@@ -445,7 +445,7 @@ class HipKernels(KernelSizes):
         self._clamps: dict = {}     # (m, n, k) -> which gated product clamps (`gemm_clamped_glu`), or 0
         self._bare: dict = {}       # (m, n, k) -> the parts that `gemm_bare` leaves such a product in, or 0
         self._float8_scratch: dict = {}      # (m, n, k, gated, full sums) -> scratch bytes of a product from rows in 8 bits
-        self._float8_experts: dict = {}      # (pairs, experts, top) -> whether few pairs' kernels take them, and whether the second sums them
+        self._float8_experts: dict = {}      # (pairs, experts, top) -> whether they are one row's, and whether the kernels of few pairs take them
         self._float8_few_rows = int(self.lib.bh_gemm_float8_few_rows())      # up to so many rows a product takes them as they are
         self.page_size = int(self.lib.bh_page_size())
         if self.page_size != _build.source_page_size():
@@ -1032,21 +1032,22 @@ class HipKernels(KernelSizes):
         act = (float(limit), float(alpha), float(shift))
         x_at, x_code, out_at, out_code = self._ptr(x, "experts x"), _code(x, "experts x"), self._ptr(out, "experts out"), _code(out, "experts out")
         through_at = self._ptr(through, "experts input", None, True)
-        in_weights, out_weights = (weights_at, None) if weigh_input else (None, weights_at)
         plan = self._float8_experts.get((pairs, experts, top))
         if plan is None:
-            plan = self._float8_experts[(pairs, experts, top)] = (bool(lib.bh_experts_float8_few(pairs, experts)), bool(lib.bh_experts_float8_sums(pairs, experts, top)))
-        few, sums = plan
-        y = None if sums else torch.empty((pairs, width), dtype=torch.float32, device=self.device)
+            plan = self._float8_experts[(pairs, experts, top)] = (bool(lib.bh_experts_float8_one(pairs, top)), bool(lib.bh_experts_float8_few(pairs, experts)))
+        one, few = plan
+        if one:
+            inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
+            self._check(lib.bh_experts_float8_row(
+                x_at, x_code, chosen_at, weights_at, int(weigh_input), through_at, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), w_down.data.data_ptr(),
+                w_down.scales.data_ptr(), inner.data_ptr(), out_at, out_code, top, k, ff, width, *act, int(bool(fresh)), int(full_up), int(full), stream))
+            return
+        in_weights, out_weights = (weights_at, None) if weigh_input else (None, weights_at)
+        y = torch.empty((pairs, width), dtype=torch.float32, device=self.device)
         if few:
             inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
             self._check(lib.bh_experts_float8_rows(x_at, x_code, top, chosen_at, pairs, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(),
                                                    ff, k, 1, *act, in_weights, int(full_up), stream))
-            if sums:
-                self._check(lib.bh_experts_float8_rows_sum(inner.data_ptr(), chosen_at, out_weights, through_at, x_code, w_down.data.data_ptr(),
-                                                           w_down.scales.data_ptr(), out_at, out_code, n, experts, top, width, ff, int(bool(fresh)), int(full),
-                                                           stream))
-                return
             self._check(lib.bh_experts_float8_rows(inner.data_ptr(), F32, 1, chosen_at, pairs, experts, w_down.data.data_ptr(), w_down.scales.data_ptr(),
                                                    y.data_ptr(), width, ff, 0, *act, None, int(full), stream))
         else:
