@@ -17,7 +17,7 @@ import sys
 import time
 
 USAGE = """usage:
-  beholdd generate --model DIR [--dtype bfloat16|float32] --prompt-ids 1,2,3 [--prompt-ids 4,5 ...]
+  beholdd generate --model DIR [--dtype bfloat16|float32] [--weights stored|float8] --prompt-ids 1,2,3 [--prompt-ids 4,5 ...]
                    [--prompt-ids-file FILE] [--max-new-tokens N] [--temperature X] [--top-k K] [--top-p P]
                    [--seed N] [--stop-token-ids a,b] [--max-tokens N] [--slots N] [--batch-size N]
                    [--max-rows-per-step N] [--logits-out PATH] [--step-timing-out PATH] [--memory-budget-bytes N] [--plan-only]
@@ -80,7 +80,7 @@ def _generate(args: list, out) -> int:
 
     flags = _parse_flags(
         args,
-        valued={"--model", "--dtype", "--prompt-ids", "--prompt-ids-file", "--max-new-tokens", "--temperature",
+        valued={"--model", "--dtype", "--weights", "--prompt-ids", "--prompt-ids-file", "--max-new-tokens", "--temperature",
                 "--top-k", "--top-p", "--seed", "--stop-token-ids", "--max-tokens", "--slots", "--batch-size",
                 "--logits-out", "--step-timing-out", "--memory-budget-bytes", "--max-rows-per-step"},
         switches={"--plan-only"}, repeatable={"--prompt-ids"})
@@ -121,7 +121,9 @@ def _generate(args: list, out) -> int:
     data, path = read_config_json(flags["--model"])
     entry = resolve_architecture(data, path)
     config = configuration_of(entry, data, path, flags["--model"])
-    dtype = flags.get("--dtype", "bfloat16")
+    dtype, kept_as = flags.get("--dtype", "bfloat16"), flags.get("--weights", "stored")
+    if kept_as not in ("stored", "float8"):
+        raise UsageError(f"--weights is stored or float8, got {kept_as}")
 
     if "--plan-only" in flags:
         import torch
@@ -132,7 +134,7 @@ def _generate(args: list, out) -> int:
         from .engine.memory import plan_memory
         from .kernels import KernelSizes
 
-        model, weights = open_model(flags["--model"], dtype, "cpu")      # the header only: no tensor is read
+        model, weights = open_model(flags["--model"], dtype, "cpu", kept_as)      # the header only: no tensor is read
         try:
             weight_bytes = weights.planned_bytes(model.tensor_specs())
         finally:
@@ -154,7 +156,7 @@ def _generate(args: list, out) -> int:
     from .engine.artifact import write_logits_artifact
 
     engine = Engine(flags["--model"], dtype=dtype, max_tokens=max_tokens, max_slots=slots,
-                    memory_limit_bytes=budget, max_rows_per_step=step_rows)
+                    memory_limit_bytes=budget, max_rows_per_step=step_rows, weights=kept_as)
     if stops is None:
         stops = list(getattr(config, "eos_token_ids", ()))
     # Without a capture the loop runs one step ahead of the host and nothing waits per token; the per-step

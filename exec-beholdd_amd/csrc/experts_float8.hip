@@ -419,7 +419,7 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
   for (int g = 0; g < Ring::G; ++g)
     ws[g] = w.scales + (((size_t)expert * Ring::G + g) * w.scale_rows() + min((tile_n * WN + wn) * HALF, blocks - 1) / 8) * steps;
   f8_f32x4_t acc[XB][YB];
-  Ring::walk(ring, from, row_at, F8_K, exponents, x_at, padded, ws, steps, acc);
+  Ring::walk(ring, from, row_at, F8_K, exponents, x_at, padded, ws, 0, steps, acc);
 
   int pair[XB];      // (read again: registers are short in the walk)
 #pragma unroll

@@ -38,12 +38,12 @@ struct F8Ring {
 
   // Where a wave's operands come from: the first ROW_PARTS addresses are those of rows, `row_step` bytes a step, the others those of its pieces
   // of the weights; row_at: a lane's own offset (16 * lane for rows in blocks), x_at: that of its row's word of exponents, four stretches
-  // `exponents_step` words behind the four before.  All of an address but the lane's offset is the same for the wave: buffer loads take it from
+  // `exponents_step` words behind the four before, from stretch `first` on (the other addresses are those of stretch `first`).  All of an address but the lane's offset is the same for the wave: buffer loads take it from
   // scalar registers, of which there are enough.  DIRECT takes rows in blocks.
   // acc[x][y][i]: row 16 (XB wm + x) + lane % 16 of the tile, weight row 16 y + 4 (lane / 16) + i of the wave's.
   __device__ static inline void walk(f8_u32x4_t* __restrict__ ring, const uint8_t* const (&from)[ROW_PARTS + W_EACH], const uint32_t (&row_at)[ROW_PARTS],
                                      int row_step, const uint32_t* exponents, const uint32_t (&x_at)[XB], uint32_t exponents_step,
-                                     const float* const (&ws)[G], int steps, f8_f32x4_t (&acc)[XB][YB]) {
+                                     const float* const (&ws)[G], int first, int steps, f8_f32x4_t (&acc)[XB][YB]) {
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
     __amdgpu_buffer_rsrc_t buffer[ROW_PARTS + W_EACH];
 #pragma unroll
@@ -84,7 +84,7 @@ struct F8Ring {
     };
     auto ask_scales = [&](int step) {
 #pragma unroll
-      for (int x = 0; x < XB; ++x) words[x] = __builtin_amdgcn_raw_buffer_load_b32(words_buffer, x_at[x] * 4, (uint32_t)(step / 4) * exponents_step * 4, 0);
+      for (int x = 0; x < XB; ++x) words[x] = __builtin_amdgcn_raw_buffer_load_b32(words_buffer, x_at[x] * 4, (uint32_t)((first + step) / 4) * exponents_step * 4, 0);
 #pragma unroll
       for (int g = 0; g < G; ++g) wsv[g] = ws[g][step];
     };
@@ -122,7 +122,7 @@ struct F8Ring {
       float s[G][XB];
 #pragma unroll
       for (int x = 0; x < XB; ++x) {
-        const float xs = f8_scale((words[x] >> (8 * (j % 4))) & 0xffu);
+        const float xs = f8_scale((words[x] >> (8 * ((first + j) % 4))) & 0xffu);
 #pragma unroll
         for (int g = 0; g < G; ++g) s[g][x] = xs * wsv[g];
       }

@@ -1,9 +1,7 @@
 // Matrix products with weights and activations in 8 bits (float8.h): C[M, N] (+)= x[M, K] * W[N, K]^T, plain or gated.
-//   few     up to 32 rows straight from bfloat16 or float32 rows (a wave quantises the stretch it multiplies), up to 64 from rows in 8 bits
-//   tiles   from rows in 8 bits (float8_rows.hip), K in parts where the tiles alone leave compute units idle
-//   rings   many rows (gemm_float8_ring.hip)
+//   few     up to 16 rows straight from bfloat16 or float32 rows (a wave quantises the stretch it multiplies), up to 128 from rows in 8 bits
+//   rings   many rows (gemm_float8_ring.hip), K in parts where the tiles alone leave compute units idle, and their sum
 #include "float8_few.h"
-#include "float8_tiles.h"
 #include "gemm_float8_ring.h"
 
 namespace {
@@ -11,7 +9,7 @@ namespace {
 // ---- a few rows ------------------------------------------------------------------------------------------------
 // Bound by reading W once, and for small W by the chain of a launch.  A workgroup owns `span` weight rows (gated: 16 pairs of gate and up);
 // its eight waves take the stretches of k in turn, each with DEPTH of them on their way, and quantise the rows' stretch themselves (16 values
-// a lane and half an operand, the largest of a stretch found between the four lanes of a row), or, from 33 rows on, read it in 8 bits.  The
+// a lane and half an operand, the largest of a stretch found between the four lanes of a row), or, from 17 rows on, read it in 8 bits.  The
 // waves' sums are added through LDS in a fixed order.
 // `span` is 16, a block of the layout; 24 where blocks of 16 are more than the compute units and fewer than twice as many, which would
 // leave some with two blocks and the others with one; 8 where they are half of the compute units or fewer.
@@ -74,18 +72,17 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict
     }
   };
   auto multiply = [&](int u) {
-    F8Operand<FULL> xo[MB];
-    float xs[MB];
+    F8Operand<FULL> wo[TT], xo;
 #pragma unroll
-    for (int b = 0; b < MB; ++b) xo[b].set(xv[u][b].quantised(&xs[b]));
+    for (int t = 0; t < TT; ++t) wo[t].set(f8_operand(wv[u][t][0], wv[u][t][1]));
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      F8Operand<FULL> wo;
-      wo.set(f8_operand(wv[u][t][0], wv[u][t][1]));
+    for (int b = 0; b < MB; ++b) {
+      float xs;
+      xo.set(xv[u][b].quantised(&xs));
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        const f8_f32x4_t sum = f8_stretch(wo, xo[b]);
-        const float s = xs[b] * wsv[u][t];
+      for (int t = 0; t < TT; ++t) {
+        const f8_f32x4_t sum = f8_stretch(wo[t], xo);
+        const float s = xs * wsv[u][t];
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t][b][e] = fmaf(sum[e], s, acc[t][b][e]);
       }
@@ -128,64 +125,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict
   }
 }
 
-// ---- tiles -----------------------------------------------------------------------------------------------------
-// Four waves of 32 rows x 64 weight rows each, operands straight from memory, the next stretch's on their way.
-// With K in parts (grid y) part p leaves its bare sums at sums + p * M * width, width = N, or 2 N of a gated product (gate, then up).
-template <typename TC, bool GATED, bool FULL, bool PARTS>
-__global__ __launch_bounds__(256) void tiles_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, F8Weight w,
-                                                    TC* __restrict__ c, int M, int ldc, int accumulate, GateForm form) {
-  constexpr int XB = 2, YB = 4, OUTS = GATED ? 64 : 128, HALF = GATED ? YB / 2 : YB;      // a wave's blocks of outputs
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / 2, wn = wave % 2;
-  const int n_tiles = (w.rows + OUTS - 1) / OUTS, tile_n = blockIdx.x % n_tiles, tile_m = blockIdx.x / n_tiles;
-  const int stretches = w.stretches, blocks = w.blocks(), row_blocks = (M + 15) / 16, padded = row_blocks * 16;
-  const int first = (int)((long)stretches * blockIdx.y / gridDim.y), end = (int)((long)stretches * (blockIdx.y + 1) / gridDim.y);
-  const uint8_t* ap[XB];
-  const uint8_t* wp[YB];
-  const float* ws[YB];
-  const uint32_t* xp[XB];
-#pragma unroll
-  for (int x = 0; x < XB; ++x) {
-    const int block = min((tile_m * 2 + wm) * XB + x, row_blocks - 1);
-    ap[x] = a + (size_t)block * stretches * F8_BLOCK + lane * 16;
-    xp[x] = exponents + block * 16 + lane % 16;
-  }
-#pragma unroll
-  for (int y = 0; y < YB; ++y) {
-    const int block = min((tile_n * 2 + wn) * HALF + y % HALF, blocks - 1), matrix = y / HALF;
-    wp[y] = w.data + ((size_t)matrix * blocks + block) * stretches * F8_BLOCK + lane * 16;
-    ws[y] = w.scales + ((size_t)matrix * w.scale_rows() + block / 8) * stretches;
-  }
-  f8_f32x4_t acc[XB][YB];
-#pragma unroll
-  for (int x = 0; x < XB; ++x)
-#pragma unroll
-    for (int y = 0; y < YB; ++y) acc[x][y] = f8_f32x4_t{0.f, 0.f, 0.f, 0.f};
-  f8_walk<FULL, XB, YB, F8_BLOCK, 1024>(ap, xp, padded, wp, ws, first, end, acc);
-  const int N = w.rows;
-#pragma unroll
-  for (int x = 0; x < XB; ++x) {
-    const int row = ((tile_m * 2 + wm) * XB + x) * 16 + lane % 16;
-    if (row >= M) continue;
-#pragma unroll
-    for (int y = 0; y < (PARTS ? YB : HALF); ++y) {
-      const int n = ((tile_n * 2 + wn) * HALF + y % HALF) * 16 + 4 * (lane / 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= N) break;
-        if constexpr (PARTS) {
-          const int width = GATED ? 2 * N : N;
-          reinterpret_cast<float*>(c)[((size_t)blockIdx.y * M + row) * width + (y / HALF) * N + n + e] = acc[x][y][e];
-        } else {
-          TC* at = c + (size_t)row * ldc + n + e;
-          float value = GATED ? gate_mul(acc[x][y][e], acc[x][y + (GATED ? HALF : 0)][e], form) : acc[x][y][e];
-          if (accumulate) value += to_f32(*at);
-          *at = from_f32<TC>(value);
-        }
-      }
-    }
-  }
-}
-
+// ---- K in parts ------------------------------------------------------------------------------------------------
 // The parts' sums in their order.  grid (ceil(N / 256), M).
 template <typename TC, bool GATED>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ sums, TC* __restrict__ c, int parts, int N, int ldc, int accumulate,
@@ -205,16 +145,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS = 32, FEW_ROWS_IN_8 = 64, MOST_PARTS = 16;
-
-int parts_of(int M, int N, int K, bool gated) {
-  const long tiles = (long)((M + 63) / 64) * ((N + (gated ? 63 : 127)) / (gated ? 64 : 128));
-  const int stretches = (K + F8_K - 1) / F8_K;
-  const long units = 2L * bh_compute_units();
-  const int wanted = (int)(tiles >= units ? 1 : (units + tiles - 1) / tiles);
-  const int most = stretches / 4 < MOST_PARTS ? stretches / 4 : MOST_PARTS;
-  return wanted < most ? wanted : most > 1 ? most : 1;
-}
+constexpr int FEW_ROWS = 16, FEW_ROWS_IN_8 = 128;
 
 int span_of(int N, int K, bool gated) {
   if (gated) return 16;
@@ -233,14 +164,14 @@ void launch_few_blocks(const void* x, const uint32_t* exponents, const F8Weight&
 #define BH_F8_FEW(NB, LOAD, MASKED, DEPTH)                                                                                            \
   few_kernel<T, TC, MB, NB, GATED, FULL, LOAD, MASKED, DEPTH><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)x, exponents, w, c, M, K, \
                                                                                                    ldc, accumulate, span, form)
-  constexpr int DEPTH = MB == 1 && !GATED ? 4 : MB <= 2 && sizeof(T) <= 2 ? 3 : 2;
+  constexpr int DEPTH = MB == 1 && !GATED ? 4 : MB <= 2 && sizeof(T) <= 2 ? 3 : MB <= 6 ? 2 : 1;
   if constexpr (SPANS) {
     if (span == 8) {
       BH_F8_FEW(1, F8_EVEN, true, DEPTH);
       return;
     }
     if (span == 24) {
-      BH_F8_FEW(2, F8_EVEN, true, (MB == 1 ? 4 : 2));
+      BH_F8_FEW(2, F8_EVEN, true, (MB == 1 ? 4 : MB <= 4 ? 2 : 1));
       return;
     }
   }
@@ -256,23 +187,15 @@ template <typename T, typename TC, bool GATED, bool FULL>
 void launch_few(const void* x, const uint32_t* exponents, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
 #define BH_F8_FEW(MB) launch_few_blocks<T, TC, GATED, FULL, MB>(x, exponents, w, c, M, K, ldc, accumulate, form, stream)
   if constexpr (sizeof(T) == 1) {
-    if (M <= 48) BH_F8_FEW(3);
-    else BH_F8_FEW(4);
-  } else if (M <= 16) BH_F8_FEW(1);
-  else BH_F8_FEW(2);
-#undef BH_F8_FEW
-}
-
-template <typename TC, bool GATED, bool FULL>
-void launch_tiles(const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, float* sums, int parts, int M, int ldc, int accumulate,
-                  GateForm form, hipStream_t stream) {
-  const dim3 grid((unsigned)(((long)(M + 63) / 64) * ((w.rows + (GATED ? 63 : 127)) / (GATED ? 64 : 128))), parts);
-  if (parts == 1) {
-    tiles_kernel<TC, GATED, FULL, false><<<grid, 256, 0, stream>>>(a, exponents, w, c, M, ldc, accumulate, form);
-    return;
+    if (M <= 32) BH_F8_FEW(2);
+    else if (M <= 48) BH_F8_FEW(3);
+    else if (M <= 64) BH_F8_FEW(4);
+    else if (M <= 96) BH_F8_FEW(6);
+    else BH_F8_FEW(8);
+  } else {
+    BH_F8_FEW(1);
   }
-  tiles_kernel<float, GATED, FULL, true><<<grid, 256, 0, stream>>>(a, exponents, w, sums, M, ldc, 0, form);
-  finish_kernel<TC, GATED><<<dim3((w.rows + 255) / 256, M), 256, 0, stream>>>(sums, c, parts, w.rows, ldc, accumulate, form);
+#undef BH_F8_FEW
 }
 
 int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int M, int N, int K, int ldc, int gate) {
@@ -290,9 +213,9 @@ int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int 
 extern "C" int bh_gemm_float8_few_rows() { return FEW_ROWS; }
 // Bytes of scratch memory of a product from rows in 8 bits.
 extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full) {
-  if (M <= FEW_ROWS_IN_8 || N <= 0 || K <= 0 || float8_ring_tile(M, N, K, gated != 0, full != 0) >= 0) return 0;
-  const int parts = parts_of(M, N, K, gated != 0);
-  return parts > 1 ? (long)parts * M * N * (gated ? 2 : 1) * 4 : 0;
+  if (M <= FEW_ROWS_IN_8 || N <= 0 || K <= 0) return 0;
+  const F8RingPlan plan = float8_ring_plan(M, N, K, gated != 0, full != 0);
+  return plan.parts > 1 ? (long)plan.parts * M * N * (gated ? 2 : 1) * 4 : 0;
 }
 
 #define BH_F8_BY_TYPES(RUN)                                                                                        \
@@ -335,17 +258,18 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
 #undef BH_F8_RUN
     return bh_check_launch("gemm_float8");
   }
-  const int tile = float8_ring_tile(M, N, K, gate != 0, full != 0);
-  if (tile >= 0)
-    return float8_ring_launch(tile, (const uint8_t*)a, (const uint32_t*)exponents, {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K}, c,
-                              c_dtype, accumulate, M, ldc, gate != 0, full, bh_gate_form(gate), stream);
-  const int parts = parts_of(M, N, K, gate != 0);
-  BH_REQUIRE(parts == 1 || scratch != nullptr, "gemm_float8: a product in %d parts needs scratch memory", parts);
+  const F8RingPlan plan = float8_ring_plan(M, N, K, gate != 0, full != 0);
+  BH_REQUIRE(plan.parts == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), "gemm_float8: a product in %d parts needs scratch memory", plan.parts);
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
   const GateForm form = bh_gate_form(gate);
-#define BH_F8_RUN(TC, GATED, FULL) \
-  launch_tiles<TC, GATED, FULL>((const uint8_t*)a, (const uint32_t*)exponents, weight, (TC*)c, (float*)scratch, parts, M, ldc, accumulate, form, stream)
-  BH_F8_BY_TYPES(BH_F8_RUN);
-#undef BH_F8_RUN
+  const int status = float8_ring_launch(plan, (const uint8_t*)a, (const uint32_t*)exponents, weight, c, c_dtype, (float*)scratch, accumulate, M, ldc, gate != 0, full,
+                                        form, stream);
+  if (status != 0 || plan.parts == 1) return status;
+  const dim3 grid((N + 255) / 256, M);
+  if (c_dtype == BH_F32) {
+    if (gate) finish_kernel<float, true><<<grid, 256, 0, stream>>>((const float*)scratch, (float*)c, plan.parts, N, ldc, accumulate, form);
+    else finish_kernel<float, false><<<grid, 256, 0, stream>>>((const float*)scratch, (float*)c, plan.parts, N, ldc, accumulate, form);
+  } else if (gate) finish_kernel<bf16_t, true><<<grid, 256, 0, stream>>>((const float*)scratch, (bf16_t*)c, plan.parts, N, ldc, accumulate, form);
+  else finish_kernel<bf16_t, false><<<grid, 256, 0, stream>>>((const float*)scratch, (bf16_t*)c, plan.parts, N, ldc, accumulate, form);
   return bh_check_launch("gemm_float8");
 }

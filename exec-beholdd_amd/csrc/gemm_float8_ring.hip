@@ -29,14 +29,17 @@ __device__ inline void tile_of_workgroup(int n_tiles, int m_tiles, int* tile_n, 
 }
 
 // A tile that sticks out of the matrix repeats its last blocks and stores only what exists.
-template <typename TC, bool GATED, bool FULL, int XB, int YB, int WM, int WN, int R, bool DIRECT, int BM, int BN>
+// With K in parts (PARTS, grid y) part p leaves its bare sums at c + p * M * width, width = N, or 2 N of a gated product (gate, then up).
+template <typename TC, bool GATED, bool FULL, bool PARTS, int XB, int YB, int WM, int WN, int R, bool DIRECT, int BM, int BN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, F8Weight w,
                                                                      TC* __restrict__ c, int M, int ldc, int accumulate, GateForm form) {
   using Ring = F8Ring<FULL, XB, YB, WM, WN, R, GATED ? 2 : 1, DIRECT>;
   constexpr int HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS;
   __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[R * Ring::PIECES * 64];      // [step in turn][A's pieces, then W's][lane]
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
-  const int N = w.rows, steps = w.stretches, blocks = w.blocks(), row_blocks = (M + 15) / 16, padded = row_blocks * 16;
+  const int N = w.rows, stretches = w.stretches, blocks = w.blocks(), row_blocks = (M + 15) / 16, padded = row_blocks * 16;
+  const int first = PARTS ? (int)((long)stretches * blockIdx.y / gridDim.y) : 0;
+  const int steps = PARTS ? (int)((long)stretches * (blockIdx.y + 1) / gridDim.y) - first : stretches;
   int tile_n, tile_m;
   tile_of_workgroup<BM, BN>((N + OUTS - 1) / OUTS, (M + ROWS - 1) / ROWS, &tile_n, &tile_m);
   const uint8_t* from[Ring::ROW_PARTS + Ring::W_EACH];
@@ -44,14 +47,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
 #pragma unroll
   for (int i = 0; i < Ring::ROW_PARTS; ++i) {
     const int piece = DIRECT ? 2 * (wm * XB + i) : wave * Ring::A_EACH + i;
-    from[i] = a + (size_t)min(tile_m * (XB * WM) + piece / 2, row_blocks - 1) * steps * F8_BLOCK + piece % 2 * 1024;
+    from[i] = a + ((size_t)min(tile_m * (XB * WM) + piece / 2, row_blocks - 1) * stretches + first) * F8_BLOCK + piece % 2 * 1024;
     row_at[i] = lane * 16;
   }
 #pragma unroll
   for (int i = 0; i < Ring::W_EACH; ++i) {
     const int piece = wave * Ring::W_EACH + i, b = piece / 2, column = b / YB, y = b % YB;
     const int block = min((tile_n * WN + column) * HALF + y % HALF, blocks - 1);
-    from[Ring::ROW_PARTS + i] = w.data + ((size_t)(y / HALF) * blocks + block) * steps * F8_BLOCK + piece % 2 * 1024;
+    from[Ring::ROW_PARTS + i] = w.data + (((size_t)(y / HALF) * blocks + block) * stretches + first) * F8_BLOCK + piece % 2 * 1024;
   }
   uint32_t x_at[XB];
 #pragma unroll
@@ -59,9 +62,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
   const float* ws[Ring::G];
 #pragma unroll
   for (int g = 0; g < Ring::G; ++g)
-    ws[g] = w.scales + ((size_t)g * w.scale_rows() + min((tile_n * WN + wn) * HALF, blocks - 1) / 8) * steps;
+    ws[g] = w.scales + ((size_t)g * w.scale_rows() + min((tile_n * WN + wn) * HALF, blocks - 1) / 8) * stretches + first;
   f8_f32x4_t acc[XB][YB];
-  Ring::walk(ring, from, row_at, F8_BLOCK, exponents, x_at, padded, ws, steps, acc);
+  Ring::walk(ring, from, row_at, F8_BLOCK, exponents, x_at, padded, ws, first, steps, acc);
 
   const bool fours = (N | ldc) % 4 == 0 && (uintptr_t)c % (4 * sizeof(TC)) == 0;
 #pragma unroll
@@ -69,13 +72,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
     const int row = tile_m * ROWS + (wm * XB + x) * 16 + lane % 16;
     if (row >= M) continue;
 #pragma unroll
-    for (int y = 0; y < HALF; ++y) {
-      const int n = ((tile_n * WN + wn) * HALF + y) * 16 + 4 * (lane / 16);
+    for (int y = 0; y < (PARTS ? YB : HALF); ++y) {
+      const int n = ((tile_n * WN + wn) * HALF + y % HALF) * 16 + 4 * (lane / 16);
       if (n >= N) continue;
+      if constexpr (PARTS) {
+        const size_t width = GATED ? 2 * (size_t)N : N;
+        float* sums = reinterpret_cast<float*>(c) + ((size_t)blockIdx.y * M + row) * width + (size_t)(y / HALF) * N + n;
+        if (N % 4 == 0) {
+          store_four(sums, acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) sums[e] = acc[x][y][e];
+        }
+        continue;
+      }
       TC* at = c + (size_t)row * ldc + n;
       float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = GATED ? gate_mul(acc[x][y][e], acc[x][y + (GATED ? HALF : 0)][e], form) : acc[x][y][e];
+      for (int e = 0; e < 4; ++e) v[e] = GATED ? gate_mul(acc[x][y][e], acc[x][(y + (GATED ? HALF : 0)) % YB][e], form) : acc[x][y][e];
       if (fours) {
         if (accumulate) {
           const float4 old = load_four(at);
@@ -91,35 +106,83 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
   }
 }
 
+// A tile's sizes, how many of its workgroups share a compute unit, what a step of 128 k costs a compute unit that has one of them, or two, and what
+// their start and end cost, with the matrix cores' own sums and with full ones (us).  From the times of every tile and cut of K for 9 products of 129
+// to 8,160 rows, 1,024 to 24,576 weight rows and k of 1,000 to 12,288 (94 sizes, 1,300 times): what this chooses there takes 1 % longer than the best
+// of them on average, 11 % at most.  Where the tiles are ahead, us, 64 x 256 / 128 x 128 / 256 x 128 / 256 x 256: 512 rows of 4,096 x 4,096 21.1 / 28.7 /
+// 33 / 55; 2,048 rows 45.3 / 39.6 / 41.5 / 57; 4,096 rows 88 / 75.6 / 81.4 / 69.8; 200 rows of 12,288 k in four parts 26.3, in one 55.
 struct TileShape {
-  int rows, columns;      // of weight rows
+  int rows, columns, share;
+  double step, step_shared, start_and_end, full_step, full_step_shared, full_start_and_end;
 };
-constexpr TileShape SHAPES[] = {{128, 128}, {256, 128}, {256, 256}};
+constexpr TileShape SHAPES[] = {{128, 128, 2, 0.755, 1.122, 3.5, 1.163, 1.637, 6.8},
+                                {256, 128, 1, 0.861, 0., 6.3, 1.545, 0., 9.5},
+                                {256, 256, 1, 1.489, 0., 9.8, 0., 0., 0.},
+                                {64, 256, 1, 0.561, 0., 4.3, 0.944, 0., 5.4},
+                                {128, 256, 1, 0.863, 0., 6.4, 1.555, 0., 9.2}};
+constexpr int TILES = 5, MOST_PARTS = 8;
 
-template <typename TC, bool GATED, bool FULL>
-void launch(int tile, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, int accumulate, int M, int ldc, GateForm form, hipStream_t stream) {
+double cost_us(int tile, int parts, int M, int W, int K, bool full) {
+  const TileShape& s = SHAPES[tile];
+  const long units = bh_compute_units(), workgroups = (long)((M + s.rows - 1) / s.rows) * ((W + s.columns - 1) / s.columns) * parts;
+  const double steps = ((K + F8_K - 1) / F8_K + parts - 1) / parts;
+  const double ends = full ? s.full_start_and_end : s.start_and_end;
+  const double alone = steps * (full ? s.full_step : s.step) + ends, both = steps * (full ? s.full_step_shared : s.step_shared) + ends;
+  double t;
+  if (s.share == 1) {
+    t = (double)((workgroups + units - 1) / units) * alone;
+  } else {      // whole rounds of two a compute unit, then a last one: of two, which take as long on some units as on all, or of one
+    const long rest = workgroups % (2 * units);
+    t = (double)(workgroups / (2 * units)) * both + (rest > units ? both : rest > 0 ? alone : 0.);
+  }
+  if (parts == 1) return t;
+  return t + 4.0 + parts * (double)M * W * 8.0 / 7.3e6;      // the parts' sums on their way to memory and back, and a launch
+}
+
+template <typename TC, bool GATED, bool FULL, bool PARTS>
+void launch(int tile, int parts, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, int accumulate, int M, int ldc, GateForm form,
+            hipStream_t stream) {
   const int outs = SHAPES[tile].columns / (GATED ? 2 : 1), rows = SHAPES[tile].rows;
-  const dim3 grid((unsigned)(((w.rows + outs - 1) / outs) * (long)((M + rows - 1) / rows)));
-#define BH_F8_RING(FULL, XB, YB, WM, WN, R, DIRECT, BM, BN) \
-  float8_ring_kernel<TC, GATED, FULL, XB, YB, WM, WN, R, DIRECT, BM, BN><<<grid, 64 * WM * WN, 0, stream>>>(a, exponents, w, c, M, ldc, accumulate, form)
+  const dim3 grid((unsigned)(((w.rows + outs - 1) / outs) * (long)((M + rows - 1) / rows)), parts);
+#define BH_F8_RING(FULL, XB, YB, WM, WN, R, DIRECT, BM, BN)                                                                             \
+  float8_ring_kernel<TC, GATED, FULL, PARTS, XB, YB, WM, WN, R, DIRECT, BM, BN><<<grid, 64 * WM * WN, 0, stream>>>(a, exponents, w, c, M, \
+                                                                                                                  ldc, accumulate, form)
   if (tile == 0) BH_F8_RING(FULL, 4, 4, 2, 2, 2, false, 8, 8);
   else if (tile == 1) BH_F8_RING(FULL, 4, 4, 4, 2, 3, false, 8, 4);
-  else if constexpr (!FULL) BH_F8_RING(false, 4, 8, 4, 2, 3, true, 8, 4);
+  else if (tile == 3) BH_F8_RING(FULL, 2, 4, 2, 4, 3, false, 8, 4);
+  else if (tile == 4) BH_F8_RING(FULL, 4, 4, 2, 4, 3, false, 8, 4);
+  else if constexpr (!FULL && !PARTS) BH_F8_RING(false, 4, 8, 4, 2, 3, true, 8, 4);
 #undef BH_F8_RING
+}
+
+template <typename TC, bool GATED, bool FULL>
+void launch_plan(const F8RingPlan& plan, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, float* sums, int accumulate, int M, int ldc,
+                 GateForm form, hipStream_t stream) {
+  if (plan.parts == 1) launch<TC, GATED, FULL, false>(plan.tile, 1, a, exponents, w, c, accumulate, M, ldc, form, stream);
+  else launch<float, GATED, FULL, true>(plan.tile, plan.parts, a, exponents, w, sums, 0, M, ldc, form, stream);
 }
 
 }  // namespace
 
-int float8_ring_tile(int M, int N, int K, bool gated, bool full) {
-  if (M <= 128 || K < 4 * F8_K) return -1;
-  const long wide = (long)((M + 255) / 256) * ((N * (gated ? 2L : 1L) + 127) / 128);
-  if (!full && wide >= 2L * bh_compute_units()) return 2;
-  return wide >= bh_compute_units() ? 1 : 0;
+F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full) {
+  F8RingPlan plan = {0, 1};
+  double least = 0.;
+  const int W = gated ? 2 * N : N, stretches = (K + F8_K - 1) / F8_K;
+  for (int tile = 0; tile < TILES; ++tile) {
+    if (tile == 2 && full) continue;      // (full sums have no registers for it)
+    const long tiles = (long)((M + SHAPES[tile].rows - 1) / SHAPES[tile].rows) * ((W + SHAPES[tile].columns - 1) / SHAPES[tile].columns);
+    const int most = tile == 2 || M > 65535 || tiles >= 2L * bh_compute_units() ? 1 : MOST_PARTS;
+    for (int parts = 1; parts <= most && (parts == 1 || stretches >= 4 * parts); ++parts) {
+      const double cost = cost_us(tile, parts, M, W, K, full);
+      if (least == 0. || cost < least) least = cost, plan = {tile, parts};
+    }
+  }
+  return plan;
 }
 
-int float8_ring_launch(int tile, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, void* c, int c_dtype, int accumulate, int M, int ldc,
-                       int gated, int full, GateForm form, hipStream_t stream) {
-#define BH_F8_RUN(TC, GATED, FULL) launch<TC, GATED, FULL>(tile, a, exponents, w, (TC*)c, accumulate, M, ldc, form, stream)
+int float8_ring_launch(const F8RingPlan& plan, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, void* c, int c_dtype, float* sums, int accumulate,
+                       int M, int ldc, int gated, int full, GateForm form, hipStream_t stream) {
+#define BH_F8_RUN(TC, GATED, FULL) launch_plan<TC, GATED, FULL>(plan, a, exponents, w, (TC*)c, sums, accumulate, M, ldc, form, stream)
 #define BH_F8_FULL(TC, GATED)               \
   do {                                      \
     if (full) BH_F8_RUN(TC, GATED, true);   \

@@ -54,12 +54,16 @@ class Engine:
     the cache, the largest step's temporaries and logits, the sampler and the captured decode steps.
     `memory_limit_bytes` bounds that plan's total and is checked from the checkpoint's header and the sizes
     alone, before a tensor is read or the cache allocated (the reference enforces its limits before any I/O,
-    crates/beholdd-model/src/qwen3moe/recorded_attention.rs:344-365)."""
+    crates/beholdd-model/src/qwen3moe/recorded_attention.rs:344-365).
+    `weights="float8"` keeps the matrices of the layers in 8-bit floating point with a scale for each block of 128 x 128, made from the
+    checkpoint's as it is loaded, and brings the rows that are multiplied with them into 8 bits too, a scale for each 128 values; the embedding,
+    the head, routers, norms and small tables stay as they are.  Half the bytes of bfloat16 to keep and to read in every step, at results that
+    differ from the stored weights' by the roundings to 8 bits (2^-4 of a value at most)."""
 
     def __init__(self, model_dir: str | None = None, dtype="bfloat16", max_tokens: int = 4096,
                  max_slots: int | None = None, device="cuda:0", kernels=None, model=None,
                  memory_limit_bytes: int | None = None, use_graphs: bool = True,
-                 max_rows_per_step: int | None = None, graph_limit: int = GRAPH_LIMIT, graph_rows_per_sequence: int = 1):
+                 max_rows_per_step: int | None = None, graph_limit: int = GRAPH_LIMIT, graph_rows_per_sequence: int = 1, weights: str = "stored"):
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
         if kernels is None:
@@ -74,6 +78,8 @@ class Engine:
             if isinstance(value, bool) or not isinstance(value, numbers.Integral) or value < least:
                 raise ValueError(f"{name} is an integer of at least {least}{' or None' if optional else ''}, got {value!r}")
         with_graphs = bool(use_graphs and self.device.type == "cuda")
+        if model is not None and weights != "stored":
+            raise ValueError("a built model keeps its weights as it was built: weights='float8' goes with a model folder")
 
         def make_cache(built):
             return SequenceCache(built.entry_needs, max_tokens, self.dtype, self.device, kernels.page_size,
@@ -98,14 +104,16 @@ class Engine:
         if model is None:
             if model_dir is None:
                 raise ValueError("give a model folder or a built model")
-            model, weights = open_model(model_dir, self.dtype, self.device)
+            model, bound = open_model(model_dir, self.dtype, self.device, weights)
             try:
-                self.weight_bytes = weights.planned_bytes(model.tensor_specs())
+                if weights == "float8" and not hasattr(kernels, "pack_float8"):
+                    raise ValueError("these kernels keep no weights in 8 bits")
+                self.weight_bytes = bound.planned_bytes(model.tensor_specs())
                 self.cache = make_cache(model)
                 within_budget(self.weight_bytes, self.cache)
-                model.load(weights, self.device)
+                model.load(bound, self.device)
             finally:
-                weights.reader.close()
+                bound.reader.close()
         else:
             self.weight_bytes = sum(t.numel() * t.element_size() for t in _model_tensors(model))
             self.cache = make_cache(model)
@@ -251,14 +259,24 @@ def _model_tensors(model):
     return out
 
 
-def open_model(model_dir: str, dtype, device):
+WEIGHTS = ("stored", "float8")      # how an engine keeps the layers' matrices
+
+
+def open_model(model_dir: str, dtype, device, weights: str = "stored"):
     """config.json -> architecture -> model (no tensors yet), and the checkpoint's tensors bound to it by name
-    with nothing read yet.  The caller loads (`model.load(weights, device)`) and closes `weights.reader`."""
+    with nothing read yet.  The caller loads (`model.load(weights, device)`) and closes `weights.reader`.  `weights`: how the layers'
+    matrices will be kept ("stored" or "float8")."""
     dtype = parse_dtype(dtype)
+    if weights not in WEIGHTS:
+        raise ValueError(f"weights are kept as one of {WEIGHTS}, got {weights!r}")
     data, path = read_config_json(model_dir)
     entry = resolve_architecture(data, path)
     config = configuration_of(entry, data, path, model_dir)
     model = entry.build(config)
+    if weights == "float8":
+        if not hasattr(model, "keep_in_float8"):
+            raise ValueError(f"{type(model).__name__} keeps no weights in 8 bits")
+        model.keep_in_float8()
     return model, bind(model.tensor_specs(), model_dir, dtype, device)
 
 

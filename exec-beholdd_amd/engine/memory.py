@@ -75,6 +75,13 @@ def weights_as_kept(model, act_size: int, sizes) -> tuple:
             continue
         rows, cols = linear.out_features, linear.in_features
         packs = bool(getattr(linear, "packs", lambda size: False)(act_size))
+        if getattr(linear, "float8", 0):
+            kept += sizes.float8_bytes(linear.float8, rows // linear.float8, cols) if sizes is not None else rows * cols
+            # the stacked matrix while it is loaded; later its 8-bit form beside it, and what that takes on the way
+            transient = max(transient, _rounded(rows * cols * act_size) if len(linear.names) > 1 else 0,
+                            (sizes.float8_bytes(linear.float8, rows // linear.float8, cols) + sizes.float8_packing_bytes(rows, cols)) if sizes is not None else 0)
+            in_linears.update(linear.names)
+            continue
         size = sizes.packed_bytes(rows, cols, act_size) if (packs and sizes is not None) else _rounded(rows * cols * act_size)
         kept += size
         transient = max(transient, size if (packs or len(linear.names) > 1) else 0)

@@ -114,7 +114,7 @@ class Float8Weight:
     values in blocks of 16 rows x 128 columns in matrix-core operand order (csrc/float8.h), `scales` is [matrices, blocks of rows,
     blocks of columns].  `shape` is that of the stacked matrices."""
 
-    BLOCK = 128
+    PACKED_AT_ONCE = 1024      # rows that are brought into 8 bits together
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, matrices: int, rows: int, cols: int):
         self.data, self.scales, self.matrices, self.rows = data, scales, int(matrices), int(rows)
@@ -356,6 +356,29 @@ class KernelSizes:
         if swiglu and n % 16:
             total += _rounded(m * 2 * n * act_size)
         return total
+
+    def gemm_float8_working_bytes(self, m, n, k, act_size, gated=False) -> int:
+        """Bytes that a product with an 8-bit weight allocates beside its output (n rows of one of the weight's matrices): the rows in plain
+        order where they come in blocks, the rows in 8 bits, and the sums of K in parts."""
+        m, n, k = int(m), int(n), int(k)
+        total = _rounded(m * k * act_size)
+        if m > int(self.lib.bh_gemm_float8_few_rows()):
+            scratch = max(int(self.lib.bh_gemm_float8_scratch(m, n, k, int(bool(gated)), full)) for full in (0, 1))
+            total += sum(_rounded(size) for size in Float8Rows.bytes_of(m, k)) + _rounded(scratch)
+        return total
+
+    def float8_bytes(self, matrices, rows, cols) -> int:
+        """Device bytes of `matrices` matrices [rows, cols] as `pack_float8` keeps them."""
+        count = 1
+        for axis in Float8Weight.scale_shape(matrices, rows, cols):
+            count *= axis
+        return _rounded(Float8Weight.data_bytes(matrices, rows, cols)) + _rounded(4 * count)
+
+    @staticmethod
+    def float8_packing_bytes(rows, cols) -> int:
+        """Bytes that `pack_float8` allocates while it makes a matrix of `rows` rows: some rows of blocks in float32, their quotients by the
+        scales, and their values in and out of order."""
+        return (4 + 4 + 4 + 1 + 1) * min(-(-int(rows) // 128) * 128, Float8Weight.PACKED_AT_ONCE) * (-(-int(cols) // 128) * 128)
 
     PAGE = _build.source_page_size()
 
@@ -905,22 +928,28 @@ class HipKernels(KernelSizes):
         data = torch.empty((matrices, padded * k_blocks * 128), dtype=torch.uint8, device=self.device)
         kept = torch.empty((matrices, n_blocks, k_blocks), dtype=torch.float32, device=self.device)
         sound = torch.ones((), dtype=torch.bool, device=self.device)
+        step = Float8Weight.PACKED_AT_ONCE
         for i in range(matrices):
-            one = w[i * rows:(i + 1) * rows]
-            if scales is None:
-                whole = torch.zeros((n_blocks * 128, k_blocks * 128), dtype=torch.float32, device=self.device)
-                whole[:rows, :cols] = one
-                blocks = whole.view(n_blocks, 128, k_blocks, 128)
-                largest = blocks.abs().amax(dim=(1, 3))
-                kept[i] = torch.where(largest > 0, largest / torch.full_like(largest, 448.0), torch.ones_like(largest)).clamp(min=2.0 ** -126)
-                values = (blocks / kept[i][:, None, :, None]).view(whole.shape)[:padded].to(torch.float8_e4m3fn).view(torch.uint8)
-            else:
-                kept[i] = scales[i]
-                values = torch.zeros((padded, k_blocks * 128), dtype=torch.uint8, device=self.device)
-                values[:rows, :cols] = one.contiguous().view(torch.uint8)
-            sound &= torch.isfinite(kept[i]).all() & ~((values & 0x7f) == 0x7f).any()
-            # [block of 16 rows][block of 128 k][half h of 64][lane group q][row][16]
-            data[i] = values.view(padded // 16, 16, k_blocks, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).reshape(-1)
+            for first in range(0, rows, step):
+                one = w[i * rows + first:i * rows + min(first + step, rows)]
+                count, at = one.shape[0], slice(first // 128, -(-min(first + step, rows) // 128))
+                kept_rows = -(-count // 16) * 16
+                if scales is None:
+                    whole = torch.zeros((-(-count // 128) * 128, k_blocks * 128), dtype=torch.float32, device=self.device)
+                    whole[:count, :cols] = one
+                    blocks = whole.view(-1, 128, k_blocks, 128)
+                    largest = blocks.abs().amax(dim=(1, 3))
+                    # (a quotient by a number on the host would be a product with its reciprocal)
+                    kept[i, at] = torch.where(largest > 0, largest / torch.full_like(largest, 448.0), torch.ones_like(largest)).clamp(min=2.0 ** -126)
+                    values = (blocks / kept[i, at][:, None, :, None]).view(whole.shape)[:kept_rows].to(torch.float8_e4m3fn).view(torch.uint8)
+                else:
+                    kept[i, at] = scales[i, at]
+                    values = torch.zeros((kept_rows, k_blocks * 128), dtype=torch.uint8, device=self.device)
+                    values[:count, :cols] = one.contiguous().view(torch.uint8)
+                sound &= torch.isfinite(kept[i, at]).all() & ~((values & 0x7f) == 0x7f).any()
+                # [block of 16 rows][block of 128 k][half h of 64][lane group q][row][16]
+                order = values.view(kept_rows // 16, 16, k_blocks, 2, 4, 16).permute(0, 2, 3, 4, 1, 5)
+                data[i, first * k_blocks * 128:(first + kept_rows) * k_blocks * 128].view(order.shape).copy_(order)
         if not bool(sound):
             raise KernelError("pack_float8: the matrix or its scales hold an infinity or a NaN")
         return Float8Weight(data.view(-1), kept, matrices, rows, cols)

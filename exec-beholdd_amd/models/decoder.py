@@ -90,6 +90,19 @@ class DecoderModel:
             if hasattr(part, "build_tables"):
                 part.build_tables(device)
 
+    def keep_in_float8(self) -> list:
+        """Have the parts of the layers that can keep their matrices in 8 bits; the embedding, the head and everything else stay as they are.
+        Returns the parts' names; an error if there is none."""
+        kept = []
+        for block in self.own_blocks():
+            for part in block.parts():
+                if hasattr(part, "keep_in_float8"):
+                    part.keep_in_float8()
+                    kept.append(type(part).__name__)
+        if not kept:
+            raise ValueError("no part of this model keeps its matrices in 8 bits")
+        return kept
+
     def prepare(self, kernels):
         """After loading: parts may have the kernel library regroup their weights."""
         for part in self.parts():

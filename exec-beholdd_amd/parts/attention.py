@@ -44,6 +44,10 @@ class GQAAttention:
         self.out = Linear(q_width, hidden, prefix + "o_proj.weight")
         self.q_norm = self.k_norm = None
 
+    def keep_in_float8(self):
+        self.qkv.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.qkv.reader()    # x goes to that product and nowhere else

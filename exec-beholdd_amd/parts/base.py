@@ -46,6 +46,8 @@ count), and the same ones where it does not.  Either way the engine runs a part'
 step is launched kernel by kernel or replayed from a capture, so a state advances once per token.
 Every part may say what its forward allocates: working_bytes(step: StepSize) -> int, from sizes alone; the
 engine's byte plan adds them up before anything is allocated and names the parts that do not say.
+A part whose matrices may be kept in 8 bits offers keep_in_float8(): called before anything is loaded or planned, it has `prepare`
+keep them so (`Linear.keep_in_float8`).  Parts that do not offer it keep theirs as they are.
 A part may declare `graph_safe = True`: its forward uses only the device tensors of the step
 context (never the host_* lists, never a host-side decision that changes from step to step).
 Decode steps of a model whose parts all say so are captured and replayed as HIP graphs.  That speaks of steps
@@ -186,6 +188,11 @@ class StepSize:
         if self.sizes is None:
             return 0
         return self.sizes.gemm_working_bytes(rows, outputs, inputs, self.act_size, packed, swiglu, then_norm, bare)
+
+
+    def product_in_float8(self, rows: int, outputs: int, inputs: int, swiglu: bool = False) -> int:
+        """The same of a product whose weight is kept in 8 bits (`outputs` rows of one of its matrices)."""
+        return 0 if self.sizes is None else self.sizes.gemm_float8_working_bytes(rows, outputs, inputs, self.act_size, swiglu)
 
 
 @dataclass

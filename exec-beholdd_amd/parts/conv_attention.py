@@ -54,6 +54,10 @@ class ConvGatedAttention:
         self.out = Linear(self.gate_width, hidden, prefix + "o")
         self.q_norm = self.k_norm = self.conv_weight = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

@@ -49,6 +49,10 @@ class GatedDeltaRule:
         self.state_floats = self.n_heads * self.dim * self.vdim
         self.conv_weight = self.a_log = self.dt_bias = self.norm_weight = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

@@ -13,7 +13,12 @@ shape the activation g' * sigmoid(alpha g') * (u' + shift), an infinite limit wi
 shared expert is any feed-forward part; `scoring="softmax_all"` weighs a chosen expert by its share of the softmax over all of
 them, not renormed over the chosen; `correction` adds a learned number to every expert's score for the choice alone, the
 weight is the score without it; `identity` more experts stand behind those with matrices and hand their input through
-(no tensors and no product: `experts_combine` adds weight * h).
+(no tensors and no product: `experts_combine` adds weight * h).  `groups` more than 0 has a row use experts of `keep_groups` of as many runs of
+neighbouring experts only, judged by their best expert or the sum of their two best (`group_score` "max" or "top2"); the choice goes by score
++ correction with scores of either kind ("sigmoid" or "softmax_all"), the chosen scores are divided by their sum with `renorm`, and multiplied
+by `factor` (`kernels.route_in_groups`).
+
+With `keep_in_float8()` the experts' matrices are kept in 8 bits alone, and all of a step's pairs go through `kernels.experts_float8`.
 
 The experts' matrices are kept stacked: gate and up rows of an expert in one [2 ff, width] block, [experts, ...] in
 all.  The (row, choice) pairs are grouped by expert on the device (`experts_group`).  A step of few rows then runs a
@@ -61,6 +66,10 @@ class ClampedGLU:
         self.gate_up.load(get)
         self.down.load(get)
 
+    def keep_in_float8(self):
+        self.gate_up.keep_in_float8(2)
+        self.down.keep_in_float8()
+
     def prepare(self, kernels):
         self.gate_up.prepare(kernels)
         self.down.prepare(kernels)
@@ -97,13 +106,22 @@ class RoutedExperts:
 
     def __init__(self, hidden: int, n_experts: int, top: int, ff: int, limit: float, prefix: str, shared=None,
                  alpha: float = GATE_SLOPE, router_bias: bool = True, scoring: str = "softmax", weigh_input: bool = False,
-                 shift: float = 1.0, identity: int = 0, correction: bool = False):
+                 shift: float = 1.0, identity: int = 0, correction: bool = False, groups: int = 0, keep_groups: int | None = None,
+                 group_score: str = "top2", renorm: bool = True, factor: float = 1.0):
         if not 1 <= top <= n_experts + identity:
             raise ValueError(f"a row uses 1 to {n_experts + identity} experts, got {top}")
         if scoring not in ("softmax", "sigmoid", "softmax_all"):
             raise ValueError(f"experts are weighed by 'softmax' over the chosen, by each one's 'sigmoid' or by 'softmax_all', got {scoring!r}")
-        if correction and scoring != "softmax_all":
-            raise ValueError("a correction of the choice goes with scores over all experts")
+        if correction and scoring != "softmax_all" and not groups:
+            raise ValueError("a correction of the choice goes with scores over all experts, or with groups")
+        if groups:
+            keep_groups = groups if keep_groups is None else keep_groups
+            if groups < 0 or (n_experts + identity) % groups or not 1 <= keep_groups <= groups or top > keep_groups * ((n_experts + identity) // groups):
+                raise ValueError(f"{n_experts + identity} experts in {groups} equal groups, {keep_groups} of which give a row its {top}")
+            if scoring == "softmax" or group_score not in ("max", "top2") or router_bias:
+                raise ValueError("a router in groups scores by 'sigmoid' or 'softmax_all' without a bias on its logits, and groups by 'max' or 'top2'")
+        self.groups, self.keep_groups, self.group_score, self.renorm, self.factor = int(groups), keep_groups, group_score, bool(renorm), float(factor)
+        self.float8 = None            # in 8 bits: False until `prepare` has made them, then (gate and up, down)
         if identity and weigh_input:
             raise ValueError("identity experts are weighed on their output")
         self.identity, self.has_correction = int(identity), bool(correction)
@@ -144,6 +162,11 @@ class RoutedExperts:
         if self.shared is not None:
             self.shared.load(get)
 
+    def keep_in_float8(self):
+        self.float8 = False
+        if hasattr(self.shared, "keep_in_float8"):
+            self.shared.keep_in_float8()
+
     def prepare(self, kernels):
         """The stacked matrices stay row after row (the kernels for steps of few rows read them so).  For prompts every expert's
         matrices are kept a second time in the kernel library's own form, where it has one for them: its products of many rows
@@ -157,6 +180,11 @@ class RoutedExperts:
         self.router.prepare(kernels)
         if self.shared is not None:
             self.shared.prepare(kernels)
+        if self.float8 is not None:
+            self.float8 = (kernels.pack_float8(self.w_gate_up.view(-1, self.hidden), matrices=2 * self.n_experts),
+                           kernels.pack_float8(self.w_down.view(-1, self.ff), matrices=self.n_experts))
+            self.w_gate_up = self.w_down = None
+            return
         tiles = getattr(kernels, "experts_tiles_take", None)
         if tiles is not None and tiles(self.w_gate_up.dtype, self.hidden, self.ff) and tiles(self.w_down.dtype, self.ff, self.hidden):
             self.packed = (kernels.pack_weight(self.w_gate_up.view(-1, self.hidden)), kernels.pack_weight(self.w_down.view(-1, self.ff)))
@@ -173,6 +201,9 @@ class RoutedExperts:
             total = step.matrix(step.rows, self.WIDE_ROUTER, 4) + step.product(step.rows, self.WIDE_ROUTER, self.hidden)
         total += 2 * step.matrix(step.rows, self.top, 4)
         pairs = step.rows * self.top
+        if self.float8 is not None:      # lists of the pairs, rows and activations in 8 bits or 32, the pairs' results; the input once more as rows
+            total += step.matrix(self.n_experts + 1, pairs, 4) + 2 * step.matrix(pairs, self.ff, 4) + step.matrix(pairs, self.hidden, 4)
+            return total + 2 * step.matrix(step.rows, self.hidden) + (self.shared.working_bytes(step) if self.shared is not None else 0)
         total += step.matrix(self.n_experts, step.rows, 4) + step.matrix(pairs, self.ff) + step.matrix(pairs, self.hidden, 4)
         in_place = step.act_size == 2 and self.hidden % 64 == 0 and self.ff % 64 == 0 and self._one_launch_is_faster(pairs)
         if not in_place and step.rows > step.seqs and pairs >= self.PRODUCT_PAIRS * self.n_experts:      # a step of many rows: the pairs' inputs, gate and up
@@ -197,10 +228,21 @@ class RoutedExperts:
             logits = self.router.forward(ctx, whole, out_dtype=torch.float32)
         chosen = torch.empty((n, self.top), dtype=torch.int32, device=ctx.device)
         weights = ctx.new_f32(n, self.top)
-        if self.correction is not None:
-            routing["correction"] = self.correction
-        k.route_top_k(logits, self.router_bias, chosen, weights, **routing)
+        if self.groups:
+            k.route_in_groups(logits, self.correction, chosen, weights, scoring="sigmoid" if self.scoring == "sigmoid" else "softmax", groups=self.groups,
+                              keep=self.keep_groups, group_score=self.group_score, renorm=self.renorm, factor=self.factor,
+                              experts=self.router.out_features)
+        else:
+            if self.correction is not None:
+                routing["correction"] = self.correction
+            k.route_top_k(logits, self.router_bias, chosen, weights, **routing)
         ctx.extras["routing"] = (chosen, weights)
+        if self.float8 is not None:
+            k.experts_float8(x, chosen, weights, *self.float8, hidden, limit=self.limit, alpha=self.alpha, shift=self.shift, weigh_input=self.weigh_input,
+                             fresh=fresh, through=x if self.identity else None, full_sums=ctx.act_dtype == torch.float32)
+            if self.shared is not None:
+                self.shared.forward(ctx, whole, hidden)
+            return None
         # where the weight goes: on the expert's input (the kernels that make gate and up take it) or on its output
         act = {} if self.shift == 1.0 else {"shift": self.shift}
         ahead = dict(act, in_weights=weights) if self.weigh_input else act
@@ -305,3 +347,16 @@ def _build_routed_identity_experts(config, layer_index, prefix, shared):
     sizes = config.layers[layer_index].mlp
     return RoutedExperts(config.hidden, sizes.experts, sizes.top, sizes.expert_ff, float("inf"), prefix + "mlp.", alpha=1.0,
                          router_bias=False, scoring="softmax_all", shift=0.0, identity=sizes.identity, correction=True)
+
+
+@FEED_FORWARDS.register("routed_experts_in_groups")
+def _build_routed_experts_in_groups(config, layer_index, prefix, shared):
+    """Experts of the form Wd (silu(Wg h) * (Wu h)) in groups, of which a row may use a few, chosen by corrected sigmoid scores and weighed by
+    the scores, normed over the chosen and multiplied by a factor; a shared expert of the same form."""
+    from .mlp import SwiGLU
+
+    sizes = config.layers[layer_index].mlp
+    common = SwiGLU(config.hidden, sizes.shared_ff, prefix + "mlp.shared.", names=("gate", "up", "down")) if sizes.shared_ff else None
+    return RoutedExperts(config.hidden, sizes.experts, sizes.top, sizes.expert_ff, float("inf"), prefix + "mlp.", shared=common, alpha=1.0,
+                         router_bias=False, scoring="sigmoid", shift=0.0, correction=True, groups=sizes.groups, keep_groups=sizes.keep_groups,
+                         factor=getattr(sizes, "factor", 1.0))

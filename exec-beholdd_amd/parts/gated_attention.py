@@ -97,6 +97,10 @@ class GatedAttention:
         self.out = Linear(self.gate_width, hidden, prefix + "o")
         self.q_norm = self.k_norm = self.qkv_bias = self.sinks = self.slopes = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

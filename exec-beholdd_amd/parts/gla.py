@@ -44,6 +44,10 @@ class GatedLinearAttention:
         self.out = Linear(value_width, hidden, prefix + "o")
         self.norm_weight = self.decay_bias = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     def tensor_specs(self):
         return (self.proj.tensor_specs() + self.decay_down.tensor_specs() + self.decay_up.tensor_specs() + self.out.tensor_specs() + [
             TensorSpec(self.prefix + "a2.b", (self.n_heads * self.dim,), "norm"), TensorSpec(self.prefix + "norm", (self.vdim,), "norm")])

@@ -64,6 +64,12 @@ class LatentAttention:
         self.out = Linear(self.n_heads * self.vdim, hidden, prefix + "o")
         self.latent_weight = self.key_up = self.value_up = self.frequencies = self.query_weight = self.sinks = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        if self.query_up is not None:
+            self.query_up.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

@@ -39,6 +39,10 @@ class LightningAttention:
         self.out = Linear(value_width, hidden, prefix + "o")
         self.norm_weight = self.decay = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

@@ -30,6 +30,7 @@ class Linear:
         self.out_features = sum(self.splits) + self.padding
         self.weight = None          # a tensor, or the kernel library's packed form of it
         self.shared = False
+        self.float8 = 0             # kept in 8 bits, as so many equal matrices one below the other
 
     def tensor_specs(self):
         return [TensorSpec(name, (rows, self.in_features), "linear") for name, rows in zip(self.names, self.splits)]
@@ -54,14 +55,21 @@ class Linear:
         self.weight = weight
         self.shared = True
 
+    def keep_in_float8(self, matrices: int = 1):
+        """Have `prepare` keep the matrix in 8 bits (a scale for each block of 128 x 128), as `matrices` equal ones (2: gate rows, then up
+        rows).  Call it ahead of the byte plan."""
+        if self.out_features % int(matrices):
+            raise ValueError(f"{self.out_features} rows are not those of {matrices} equal matrices")
+        self.float8 = int(matrices)
+
     def reader(self, swiglu: bool = False) -> ProductReader:
         """This map as the only reader of an activation matrix (`swiglu`: its rows are gate rows, then up rows)."""
         return ProductReader(self.out_features // 2 if swiglu else self.out_features, swiglu,
-                             packed=self.weight is not None and not isinstance(self.weight, torch.Tensor))
+                             packed=self.weight is not None and not isinstance(self.weight, torch.Tensor) and not self.float8)
 
     def packs(self, act_size: int) -> bool:
         """Whether `prepare` regroups this matrix in an engine of that element size."""
-        return not self.shared and act_size == 2 and self.in_features % 64 == 0
+        return not self.shared and not self.float8 and act_size == 2 and self.in_features % 64 == 0
 
     def reader_for_plan(self, act_size: int, swiglu: bool = False) -> ProductReader:
         """`reader()` as it will be once the weights are loaded and prepared."""
@@ -73,18 +81,29 @@ class Linear:
         kernel library allocates on the way (`bare`: `forward_bare` may be called in place of `forward`)."""
         outputs = self.out_features // 2 if swiglu else self.out_features
         total = 0 if accumulate else step.matrix(rows, outputs, out_size)
+        if self.float8 and not self.shared:
+            return total + step.product_in_float8(rows, self.out_features // self.float8, self.in_features, swiglu)
         return total + step.product(rows, outputs, self.in_features, self.packs(step.act_size), swiglu, then_norm, bare)
 
     def prepare(self, kernels):
         """Let the kernel library regroup the matrix into the layout it reads fastest."""
-        if not self.shared and hasattr(kernels, "pack_weight"):
+        if self.shared:
+            return
+        if self.float8:
+            self.weight = kernels.pack_float8(self.weight, matrices=self.float8)
+        elif hasattr(kernels, "pack_weight"):
             self.weight = kernels.pack_weight(self.weight)
+
+    def _sums(self, ctx) -> dict:
+        """How a product in 8 bits adds up: as the matrix cores do where the activations are bfloat16 (2^-9 of a value, where those sums are
+        1.4e-5 off), in float32 in a float32 engine."""
+        return {"full_sums": ctx.act_dtype == torch.float32} if self.float8 and not self.shared else {}
 
     def forward(self, ctx, x, out=None, accumulate=False, out_dtype=None):
         """x [n, in] -> out [n, out]; with accumulate the product is added into `out`."""
         if out is None:
             out = torch.empty((x.shape[0], self.out_features), dtype=out_dtype or ctx.act_dtype, device=x.device)
-        ctx.kernels.gemm(x, self.weight, out, accumulate=accumulate)
+        ctx.kernels.gemm(x, self.weight, out, accumulate=accumulate, **self._sums(ctx))
         return out
 
     def forward_bare(self, ctx, x):
@@ -97,7 +116,7 @@ class Linear:
     def add_into(self, ctx, x, residual, then_norm=None):
         """residual += W x.  With `then_norm` (a NormRequest for the norm that reads the residual next)
         returns what the product prepared of that norm's output, or None."""
-        if then_norm is None:
-            ctx.kernels.gemm(x, self.weight, residual, accumulate=True)
+        if then_norm is None or self.float8:
+            ctx.kernels.gemm(x, self.weight, residual, accumulate=True, **self._sums(ctx))
             return None
         return ctx.kernels.gemm(x, self.weight, residual, accumulate=True, then_norm=then_norm)

@@ -25,6 +25,10 @@ class SwiGLU:
         self.gate_up = Linear(hidden, [intermediate, intermediate], [prefix + names[0], prefix + names[1]])
         self.down = Linear(intermediate, hidden, prefix + names[2])
 
+    def keep_in_float8(self):
+        self.gate_up.keep_in_float8(2)
+        self.down.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.gate_up.reader(swiglu=True)    # x goes to that product and nowhere else
@@ -86,6 +90,10 @@ class SquaredReLU:
         self.hidden, self.inner = hidden, inner
         self.up = Linear(hidden, inner, prefix + "up")
         self.down = Linear(inner, hidden, prefix + "down")
+
+    def keep_in_float8(self):
+        self.up.keep_in_float8()
+        self.down.keep_in_float8()
 
     @property
     def input_reader(self):

@@ -48,6 +48,10 @@ class MatrixMemory:
         self.state_floats = self.n_heads * ((self.vdim + 1) * self.dim + 1)      # kernels: mlstm_state_floats
         self.norm_weight = self.gate_bias = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     def tensor_specs(self):
         return self.proj.tensor_specs() + self.gates.tensor_specs() + self.out.tensor_specs() + [
             TensorSpec(self.prefix + "i.b", (self.n_heads,), "linear"), TensorSpec(self.prefix + "f.b", (self.n_heads,), "linear"),

@@ -45,6 +45,11 @@ class ParallelMixers:
     def graph_safe_rows(self):
         return graph_rows_allowed(self.mixers)
 
+    def keep_in_float8(self):
+        for mixer in self.mixers:
+            if hasattr(mixer, "keep_in_float8"):
+                mixer.keep_in_float8()
+
     def tensor_specs(self):
         return [spec for mixer in self.mixers for spec in mixer.tensor_specs()]
 

@@ -42,6 +42,10 @@ class StateSpaceScan:
         self.state_floats = self.n_heads * self.n_state * self.vdim
         self.conv_weight = self.conv_bias = self.dt_bias = self.a_log = self.d_skip = self.norm_weight = None
 
+    def keep_in_float8(self):
+        self.proj.keep_in_float8()
+        self.out.keep_in_float8()
+
     @property
     def input_reader(self):
         return self.proj.reader()

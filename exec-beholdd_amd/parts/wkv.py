@@ -45,6 +45,10 @@ class TimeMixing:
     def _linears(self):
         return [*self.projections.values(), self.decay_down, self.decay_up, self.out]
 
+    def keep_in_float8(self):
+        for linear in (*self.projections.values(), self.out):
+            linear.keep_in_float8()
+
     def tensor_specs(self):
         specs = [spec for linear in self._linears() for spec in linear.tensor_specs()]
         specs += [TensorSpec(f"{self.prefix}mu.{name}", (self.hidden,), "linear") for name in self.MIXES]
