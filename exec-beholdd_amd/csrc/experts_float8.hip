@@ -18,7 +18,7 @@ struct ExpertGate {
 __device__ inline float activated(float g, float u, const ExpertGate& gate) {
   g = fminf(g, gate.limit);
   u = fminf(fmaxf(u, -gate.limit), gate.limit);
-  return g / (1.0f + expf(-gate.alpha * g)) * (u + gate.shift);
+  return f8_gated(g, gate.alpha * g) * (u + gate.shift);
 }
 
 // ---- few -------------------------------------------------------------------------------------------------------
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
                                                               const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
                                                               F8Weight w, void* __restrict__ out, uint8_t* __restrict__ out_exponents, int out_padded,
                                                               ExpertGate gate, const float* __restrict__ in_weights) {
-  using Ring = F8Ring<FULL, XB, 4, 2, 4, 3, GATED ? 2 : 1>;
+  using Ring = F8Ring<FULL, XB, 4, 2, 4, 3, GATED ? 2 : 1, false, true>;
   constexpr int YB = Ring::YB, HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS, WN = Ring::WN;
   __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[Ring::R * Ring::PIECES * 64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
@@ -402,8 +402,8 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
 #pragma unroll
   for (int i = 0; i < Ring::A_EACH; ++i) {
     const int piece = wave * Ring::A_EACH + i;
-    from[i] = a + piece % 2 * 64;
-    row_at[i] = (uint32_t)(pairs[min(p0 + piece / 2 * 16 + lane % 16, count - 1)] / in_div) * (steps * F8_K) + 16 * (lane / 16);
+    from[i] = a;
+    row_at[i] = (uint32_t)(pairs[min(p0 + piece * 8 + lane / 8, count - 1)] / in_div) * (steps * F8_K) + 16 * ((lane % 8) ^ (lane / 8));
   }
 #pragma unroll
   for (int i = 0; i < Ring::W_EACH; ++i) {

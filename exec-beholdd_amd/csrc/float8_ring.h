@@ -23,10 +23,11 @@
 #define F8_BUFFER 0x00020000      // a buffer of bytes; the addresses are checked by the launch
 
 // FULL: float8.h.  G: matrices that a wave's weight rows are of (2: gate rows, then as many up rows).  DIRECT: a wave loads its rows of the
-// next step from memory into its other set of registers itself, and only the weights go through LDS.
-template <bool FULL_, int XB_, int YB_, int WM_, int WN_, int R_, int G_, bool DIRECT_ = false>
+// next step from memory into its other set of registers itself, and only the weights go through LDS.  LINES: rows lie one after the other, and a piece is 8 rows x 128 k, whole lines of memory, rather than
+// 16 rows x 64; the 16 bytes c of its row r lie at place c ^ r, so that 8 rows' are in different banks.
+template <bool FULL_, int XB_, int YB_, int WM_, int WN_, int R_, int G_, bool DIRECT_ = false, bool LINES_ = false>
 struct F8Ring {
-  static constexpr bool FULL = FULL_, DIRECT = DIRECT_;
+  static constexpr bool FULL = FULL_, DIRECT = DIRECT_, LINES = LINES_;
   static constexpr int XB = XB_, YB = YB_, WM = WM_, WN = WN_, R = R_, G = G_;
   static constexpr int WAVES = WM * WN, A_PIECES = DIRECT ? 0 : 2 * XB * WM, W_PIECES = 2 * YB * WN, PIECES = A_PIECES + W_PIECES;
   static constexpr int A_EACH = A_PIECES / WAVES, W_EACH = W_PIECES / WAVES, EACH = A_EACH + W_EACH, HALF = YB / G;
@@ -75,6 +76,11 @@ struct F8Ring {
                         __builtin_amdgcn_raw_buffer_load_b128(buffer[x], row_at[x] + 1024, step * row_step, 0));
     };
     auto read_a = [&](int place, int x) {
+      if constexpr (LINES) {
+        const f8_u32x4_t* block = &ring[(place * PIECES + 2 * (wm * XB + x)) * 64 + lane % 16 * 8];
+        const int first_half = (lane / 16) ^ (lane % 8);
+        return f8_operand(block[first_half], block[first_half ^ 4]);
+      }
       const f8_u32x4_t* at = &ring[(place * PIECES + 2 * (wm * XB + x)) * 64 + lane];
       return f8_operand(at[0], at[64]);
     };

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void float8_rows_kernel(const T* __restrict__ 
       float u[8];
       load_eight<T, WHOLE>(from + width, k, width, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = gate_mul(v[i][j], u[j], form);
+      for (int j = 0; j < 8; ++j) v[i][j] = f8_gate_mul(v[i][j], u[j], form);
     }
   }
 #pragma unroll
