@@ -10,7 +10,7 @@
 // Bound by the chain of `top` choices for few rows, by their instructions for many.  A choice finds the largest upper half of the scores' bits,
 // ordered as whole numbers, in six steps between registers of neighbouring lanes; only where two lanes share it (one choice in thousands, or equal
 // scores) the lower halves and the indices are compared.  Measured, us, in brackets with 64-bit scores, indices and weights handed between lanes
-// through LDS at every step: 1 row of 128 4.7 (8.8), 1,234 of 160 8.4 (11.7), 8,192 of 256 20.1 (31.7).
+// through LDS at every step: 1 row of 128 4.4 (8.8), 1,234 of 160 7.4 (11.7), 8,192 of 256 16.9 (31.7).
 #include "common.h"
 
 #define RG_MAX_TOP 32
@@ -63,7 +63,7 @@ __device__ inline double wave_sum_f64(double v) {
 template <int PER>
 __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float* __restrict__ logits, int stride, const float* __restrict__ correction,
                                                                     int32_t* __restrict__ chosen, float* __restrict__ weights, int n_rows, int E, int top,
-                                                                    int groups, int keep, int softmax, int top_two, int renorm, float factor) {
+                                                                    int groups, int keep, uint32_t per_each, int softmax, int top_two, int renorm, float factor) {
   extern __shared__ double by_of[];
   const int lane = threadIdx.x % BH_WAVE, wave = threadIdx.x / BH_WAVE, row = blockIdx.x * RG_WAVES + wave;
   if (row >= n_rows) return;      // nothing below meets other waves
@@ -121,55 +121,50 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
     const double merit = top_two && each > 1 ? best.first + best.second : best.first;
     int better = 0;      // groups ahead of this lane's
     for (int g = 0; g < groups; ++g) {
-      const double other = __shfl(merit, g * lanes, BH_WAVE);
+      const double other = of_lane(merit, g * lanes);
       better += other > merit || (other == merit && g < group) ? 1 : 0;
     }
     const unsigned long long open = __ballot(group < groups && better < keep);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = lane + i * BH_WAVE;
-      if (e < E && !((open >> (e / each * lanes)) & 1ull)) taken |= 1u << i;
+      if (e < E && !((open >> ((per_each ? (int)__umulhi((uint32_t)e, per_each) : e) * lanes)) & 1ull)) taken |= 1u << i;
     }
   }
-  double sum = 0., mine = 0.;      // lane j keeps the j-th choice
-  int mine_index = 0;
-  unsigned long long best = 0;      // of this lane's experts that may be chosen, with its score
-  double best_score = 0.;
-  int best_e = 0;
-  auto find_best = [&]() {
-    best = 0;
+  unsigned long long keys[PER];      // 0: not to be chosen (any more)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const unsigned long long key = (taken >> i) & 1u ? 0 : ordered(by[i]);
-      if (key > best) {
-        best = key;
-        best_score = score[i];
-        best_e = lane + i * BH_WAVE;
-      }
-    }
-  };
-  find_best();
+  for (int i = 0; i < PER; ++i) keys[i] = (taken >> i) & 1u ? 0 : ordered(by[i]);
+  int mine_index = 0;      // lane j keeps the j-th choice
   for (int j = 0; j < top; ++j) {
+    unsigned long long best = keys[0];
+    int best_i = 0;
+#pragma unroll
+    for (int i = 1; i < PER; ++i)
+      if (keys[i] > best) {
+        best = keys[i];
+        best_i = i;
+      }
     const uint32_t high = (uint32_t)(best >> 32), most = wave_largest(high);
     unsigned long long having = __ballot(high == most);
     if (having & (having - 1)) {      // several lanes: the lower halves decide, then the index
       const uint32_t low = high == most ? (uint32_t)best : 0u, most_low = wave_largest(low);
-      const uint32_t index = high == most && low == most_low ? (uint32_t)best_e : 0xffffffffu;
+      const uint32_t index = high == most && low == most_low ? (uint32_t)(lane + best_i * BH_WAVE) : 0xffffffffu;
       having = __ballot(index == over_wave(index, [](uint32_t a, uint32_t b) { return min(a, b); }) && high == most);
     }
-    const int winner = __builtin_amdgcn_readfirstlane(__ffsll(having) - 1);
-    const int e = __builtin_amdgcn_readlane(best_e, winner);
-    const double p = of_lane(best_score, winner);
-    sum += p;
-    if (lane == j) {
-      mine = p;
-      mine_index = e;
-    }
-    if (lane == winner) {
-      taken |= 1u << (e / BH_WAVE);
-      find_best();
-    }
+    const int winner = __builtin_amdgcn_readfirstlane(__ffsll(having) - 1), which = __builtin_amdgcn_readlane(best_i, winner);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (which == i && lane == winner) keys[i] = 0;
+    if (lane == j) mine_index = winner + which * BH_WAVE;
   }
+  double mine = 0., sum = 0.;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const double theirs = __shfl(score[i], mine_index % BH_WAVE, BH_WAVE);
+    if (mine_index / BH_WAVE == i) mine = theirs;
+  }
+  if (renorm)
+    for (int j = 0; j < top; ++j) sum += of_lane(mine, j);
   if (lane < top) {
     if (renorm) mine = sum == 0. ? 0. : mine / sum;
     chosen[(size_t)row * top + lane] = mine_index;
@@ -190,9 +185,12 @@ extern "C" int bh_route_in_groups(const float* logits, int stride, const float* 
   BH_REQUIRE(top >= 1 && top <= RG_MAX_TOP && (long)top <= (long)keep * (E / groups), "route_in_groups: 1 to min(%d, %ld) experts a row, got %d",
              RG_MAX_TOP, (long)keep * (E / groups), top);
   const dim3 grid((n_rows + RG_WAVES - 1) / RG_WAVES);
+  // e / each = the upper half of e * per_each for e < 1024: rounding 2^32 / each up adds less than 1024 / 2^32 to a quotient that is at least 1 / each
+  // below the next whole number.  (Of one expert a group 2^32 does not fit: every expert is its group's.)
+  const uint32_t per_each = E == groups ? 0u : (uint32_t)(((1ull << 32) + E / groups - 1) / (E / groups));
   const size_t lds = keep < groups ? (size_t)RG_WAVES * E * sizeof(double) : 0;
 #define BH_ROUTE(PER)                                                                                                                         \
-  route_groups_kernel<PER><<<grid, RG_WAVES * 64, lds, stream>>>(logits, stride, correction, chosen, weights, n_rows, E, top, groups, keep, \
+  route_groups_kernel<PER><<<grid, RG_WAVES * 64, lds, stream>>>(logits, stride, correction, chosen, weights, n_rows, E, top, groups, keep, per_each, \
                                                                 softmax, top_two, renorm, factor)
   if (E <= BH_WAVE) BH_ROUTE(1);
   else if (E <= 2 * BH_WAVE) BH_ROUTE(2);

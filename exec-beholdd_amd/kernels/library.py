@@ -117,6 +117,10 @@ class Float8Weight:
     PACKED_AT_ONCE = 1024      # rows that are brought into 8 bits together
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, matrices: int, rows: int, cols: int):
+        if (data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != self.data_bytes(matrices, rows, cols) or scales.dtype != torch.float32
+                or not scales.is_contiguous() or tuple(scales.shape) != self.scale_shape(matrices, rows, cols) or scales.device != data.device):
+            raise KernelError(f"{matrices} matrices of {rows} x {cols} in 8 bits have {self.data_bytes(matrices, rows, cols)} bytes and scales "
+                              f"{self.scale_shape(matrices, rows, cols)}, got {tuple(data.shape)} and {tuple(scales.shape)}")
         self.data, self.scales, self.matrices, self.rows = data, scales, int(matrices), int(rows)
         self.shape, self.dtype, self.device = (self.matrices * self.rows, int(cols)), torch.float8_e4m3fn, data.device
 
@@ -139,6 +143,11 @@ class Float8Rows:
     four exponents a word (csrc/float8.h).  `shape` is that of the matrix."""
 
     def __init__(self, data: torch.Tensor, exponents: torch.Tensor, rows: int, width: int, in_rows: bool = False):
+        data_bytes, exponent_bytes = self.bytes_of(rows, width)
+        if (data.dtype != torch.uint8 or exponents.dtype != torch.int32 or not data.is_contiguous() or not exponents.is_contiguous()
+                or data.numel() != data_bytes or 4 * exponents.numel() != exponent_bytes or data.device != exponents.device):
+            raise KernelError(f"{rows} rows of {width} in 8 bits have {data_bytes} bytes and {exponent_bytes} of exponents, got {tuple(data.shape)} and "
+                              f"{tuple(exponents.shape)}")
         self.data, self.exponents, self.in_rows = data, exponents, bool(in_rows)
         self.shape, self.dtype, self.device = (int(rows), int(width)), torch.float8_e4m3fn, data.device
 
@@ -1005,6 +1014,8 @@ class HipKernels(KernelSizes):
         full = int(out.dtype == torch.float32 if full_sums is None else bool(full_sums))
         if isinstance(out, BlockedRows):
             raise KernelError("gemm: a product with an 8-bit weight writes plain rows")
+        if w.device != self.device or a.device != self.device:
+            raise KernelError(f"gemm: rows on {a.device} and a weight on {w.device}, expected {self.device}")
         few = type(a) is torch.Tensor and m <= self._float8_few_rows
         if not few:
             if not isinstance(a, Float8Rows):
@@ -1053,6 +1064,8 @@ class HipKernels(KernelSizes):
                 or not self._goes_through(through, n, width, x.dtype)):
             raise KernelError(f"experts_float8: shapes x {tuple(x.shape)}, chosen {tuple(chosen.shape)}, weights {w_up.matrices} x {w_up.rows} x {w_up.shape[1]} "
                               f"and {experts} x {width} x {w_down.shape[1]}, out {tuple(out.shape)} do not fit")
+        if w_up.device != self.device or w_down.device != self.device:
+            raise KernelError(f"experts_float8: weights on {w_up.device} and {w_down.device}, expected {self.device}")
         if through is not None and weigh_input:
             raise KernelError("experts_float8: inputs that are handed through are weighed on their way out")
         full, full_up = out.dtype == torch.float32 if full_sums is None else bool(full_sums), full_sums is None or bool(full_sums)

@@ -64,10 +64,11 @@ def test_rows_in_8_bits_at_the_borders(k):
 
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n", [3, 40])
-def test_a_value_that_is_not_finite_makes_its_row_nan_and_no_other(k, bad, dtype, n):
+@pytest.mark.parametrize("n", [3, 40, 150])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_a_value_that_is_not_finite_makes_its_row_nan_and_no_other(k, bad, dtype, n, out_dtype):
     x, (w, held) = _rows(n, 300, dtype, 1), _weight(k, 1, 50, 300, 2)
-    whole = torch.empty((n, 50), dtype=torch.float32, device=DEVICE)
+    whole = torch.empty((n, 50), dtype=out_dtype, device=DEVICE)
     k.gemm(x.to(DEVICE), w, whole)
     x[1, 290] = bad
     out = torch.empty_like(whole)
@@ -314,6 +315,39 @@ def test_a_large_call_of_few_experts_has_lists_for_all_its_pairs(k):
     _close(out[pick], want, bound)
 
 
+def test_a_value_that_is_not_finite_reaches_its_experts_rows_alone(k):
+    for n in (1, 20, 200):
+        x, chosen, weights, packed, _ = _experts(k, n, 160, 64, 6, 2, torch.bfloat16, 3)
+        out, whole = torch.empty((n, 160), device=DEVICE), torch.empty((n, 160), device=DEVICE)
+        k.experts_float8(x.to(DEVICE), chosen.to(DEVICE), weights.to(DEVICE), *packed, whole, fresh=True)
+        x[n // 2, 7] = math.nan
+        k.experts_float8(x.to(DEVICE), chosen.to(DEVICE), weights.to(DEVICE), *packed, out, fresh=True)
+        keep = [i for i in range(n) if i != n // 2]
+        assert bool(torch.isnan(out[n // 2]).all()) and torch.equal(out[keep], whole[keep])
+
+
+def test_a_rows_result_does_not_depend_on_the_rows_beside_it_but_by_rounding(k):
+    """The same row alone, in a batch and in a prompt: the same 8 bits, sums in another order."""
+    x, (w, held) = _rows(300, 1024, torch.bfloat16, 8), _weight(k, 1, 200, 1024, 9)
+    want, bound = plain.product(plain.rows(x), plain.matrix(*held), True)
+    for n in (1, 16, 17, 100, 129, 300):
+        out = torch.empty((n, 200), device=DEVICE)
+        k.gemm(x[:n].to(DEVICE), w, out)
+        _close(out, want[:n], bound[:n], f"{n} rows")
+
+
+@pytest.mark.parametrize("m,n,width,full", [(200, 512, 2048, True), (200, 512, 2048, False), (129, 100, 5000, True), (400, 64, 12288, False), (1000, 1030, 640, False),
+                                            (2100, 300, 384, True), (700, 4000, 512, False)])
+def test_tiles_and_parts_of_k(k, m, n, width, full):
+    """Sizes that go to every tile and to K in parts, some rows of each."""
+    x, (w, held) = _rows(m, width, torch.bfloat16, 1), _weight(k, 1, n, width, 2)
+    out = torch.full((m, n), math.nan, device=DEVICE)
+    k.gemm(x.to(DEVICE), w, out, full_sums=full)
+    pick = sorted({0, 1, 63, 64, 127, 128, m // 2, m - 2, m - 1})
+    _close(out[pick], *plain.product(plain.rows(x[pick]), plain.matrix(*held), full))
+    assert bool(torch.isfinite(out).all())
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 def test_refusals(k):
@@ -331,6 +365,10 @@ def test_refusals(k):
         lambda: k.pack_float8(x.to(torch.float8_e4m3fn)), lambda: k.pack_float8(x.to(torch.float8_e4m3fn), torch.ones((1, 1, 2), device=DEVICE)),
         lambda: k.pack_float8(x.to(torch.float8_e4m3fn), torch.full((1, 1, 1), math.nan, device=DEVICE)), lambda: k.pack_float8(x[:0]),
     ]
+    from beholdd.kernels.library import Float8Rows, Float8Weight
+    refused += [lambda: Float8Weight(w.data[:-16], w.scales, 2, 32, 128), lambda: Float8Weight(w.data, w.scales[:, :, :0], 2, 32, 128),
+                lambda: Float8Weight(w.data, w.scales, 2, 48, 128), lambda: Float8Rows(w.data[:16], torch.zeros((1, 16), dtype=torch.int32, device=DEVICE), 4, 128),
+                lambda: k.gemm(x, Float8Weight(w.data.cpu(), w.scales.cpu(), 2, 32, 128), out)]
     logits, chosen, weights = torch.zeros((2, 16), device=DEVICE), torch.zeros((2, 4), dtype=torch.int32, device=DEVICE), torch.zeros((2, 4), device=DEVICE)
     for more in (dict(groups=3), dict(groups=0), dict(groups=4, keep=0), dict(groups=4, keep=5), dict(groups=8, keep=1), dict(scoring="tanh"),
                  dict(group_score="sum"), dict(experts=17), dict(experts=0)):

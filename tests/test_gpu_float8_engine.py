@@ -114,3 +114,24 @@ def test_every_architecture(name, which, dtype, tmp_path):
         want = double.step([beholdd.StepEntry(double.alloc_slot(), tokens, list(range(48)))])
         off = (got - want).norm(dim=1) / want.norm(dim=1)
         assert float(off.median()) < 0.05
+
+
+def test_the_byte_plan_bounds_what_is_allocated(tmp_path):
+    """Wide enough that matrices, not the allocator's units, are the bytes."""
+    config = dict(QWEN, hidden_size=1024, intermediate_size=2816, num_attention_heads=8, head_dim=128, num_hidden_layers=3, max_position_embeddings=1024)
+    beholdd.write_random_model(str(tmp_path), config, seed=1)
+    kept = {}
+    for weights in ("stored", "float8"):
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        engine = beholdd.Engine(str(tmp_path), dtype="bfloat16", max_tokens=1024, max_slots=4, device="cuda:0", weights=weights, max_rows_per_step=512)
+        kept[weights] = torch.cuda.memory_allocated() - before
+        slot = engine.alloc_slot()
+        engine.step([beholdd.StepEntry(slot, [3] * 500, [499])])
+        for _ in range(3):
+            engine.step([beholdd.StepEntry(slot, [7], [0])])
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - before <= engine.plan.total_bytes
+        del engine
+    assert kept["float8"] < 0.75 * kept["stored"]
