@@ -10,7 +10,8 @@
 // Bound by the chain of `top` choices for few rows, by their instructions for many.  A choice finds the largest upper half of the scores' bits,
 // ordered as whole numbers, in six steps between registers of neighbouring lanes; only where two lanes share it (one choice in thousands, or equal
 // scores) the lower halves and the indices are compared.  Measured, us, in brackets with 64-bit scores, indices and weights handed between lanes
-// through LDS at every step: 1 row of 128 4.4 (8.8), 1,234 of 160 7.4 (11.7), 8,192 of 256 16.9 (31.7).
+// through LDS at every step: 1 row of 128 3.8 (8.8), 1,234 of 160 7.0 (11.7), 8,192 of 256 15.0 (31.7), of which 7.6 are a launch and the scores,
+// 3 the groups, 3.5 the choices but the first, 1.5 the weights' sum and division.
 #include "common.h"
 
 #define RG_MAX_TOP 32
@@ -23,8 +24,7 @@ struct Two {
   double first, second;
 };
 __device__ inline Two merged(Two a, Two b) {
-  const bool mine = a.first >= b.first;
-  return {mine ? a.first : b.first, mine ? fmax(a.second, b.first) : fmax(b.second, a.first)};
+  return {fmax(a.first, b.first), fmax(fmin(a.first, b.first), fmax(a.second, b.second))};
 }
 
 // The largest (or smallest) over the wave, for every lane.
@@ -47,9 +47,12 @@ __device__ inline unsigned long long ordered(double v) {
   const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
   return bits >> 63 ? ~bits : bits | (1ull << 63);
 }
-__device__ inline double of_lane(double v, int lane) {
+// v with the lanes of a group of 16 turned by N.
+template <int N>
+__device__ inline double turned(double v) {
   const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t low = __builtin_amdgcn_readlane((int)bits, lane), high = __builtin_amdgcn_readlane((int)(bits >> 32), lane);
+  const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bits, 0x120 + N /* row_ror */, 0xf, 0xf, true);
+  const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(bits >> 32), 0x120 + N, 0xf, 0xf, true);
   return __builtin_bit_cast(double, (unsigned long long)high << 32 | low);
 }
 
@@ -116,13 +119,19 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
     const int lanes = BH_WAVE / room, group = lane / lanes;
     Two best = {none, none};
     if (group < groups)
-      for (int i = lane % lanes; i < each; i += lanes) best = merged(best, Two{by_row[group * each + i], none});
+      for (int i = lane % lanes; i < each; i += lanes) {
+        const double v = by_row[group * each + i];
+        best = {fmax(best.first, v), fmax(best.second, fmin(best.first, v))};
+      }
     for (int off = lanes / 2; off > 0; off >>= 1) best = merged(best, Two{__shfl_xor(best.first, off, BH_WAVE), __shfl_xor(best.second, off, BH_WAVE)});
-    const double merit = top_two && each > 1 ? best.first + best.second : best.first;
-    int better = 0;      // groups ahead of this lane's
-    for (int g = 0; g < groups; ++g) {
-      const double other = of_lane(merit, g * lanes);
-      better += other > merit || (other == merit && g < group) ? 1 : 0;
+    double merit = top_two && each > 1 ? best.first + best.second : best.first;
+    merit = merit == merit ? merit : none;      // (of two infinite ones)
+    int better = 0;      // groups ahead of this lane's, each of a group's lanes comparing it with some
+    for (int first = 0; first < groups; first += lanes) {
+      const int g = first + lane % lanes;
+      const double other = __shfl(merit, g * lanes % BH_WAVE, BH_WAVE);
+      const unsigned long long ahead = __ballot(g < groups && (other > merit || (other == merit && g < group)));
+      better += __popcll((ahead >> (group * lanes)) & (~0ull >> (BH_WAVE - lanes)));
     }
     const unsigned long long open = __ballot(group < groups && better < keep);
 #pragma unroll
@@ -134,16 +143,36 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
   unsigned long long keys[PER];      // 0: not to be chosen (any more)
 #pragma unroll
   for (int i = 0; i < PER; ++i) keys[i] = (taken >> i) & 1u ? 0 : ordered(by[i]);
+  // Up to four experts a lane stand in order, largest first (neighbours change places, so equal ones stay in theirs), and a choice looks at the
+  // first alone; more are looked through every time.
+  constexpr bool SORTED = PER <= 4;
+  int at[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) at[i] = i;
+  if constexpr (SORTED) {
+#pragma unroll
+    for (int last = PER - 1; last > 0; --last)
+#pragma unroll
+      for (int i = 0; i < last; ++i) {
+        const bool change = keys[i + 1] > keys[i];
+        const unsigned long long key = keys[i];
+        const int index = at[i];
+        keys[i] = change ? keys[i + 1] : key, at[i] = change ? at[i + 1] : index;
+        keys[i + 1] = change ? key : keys[i + 1], at[i + 1] = change ? index : at[i + 1];
+      }
+  }
   int mine_index = 0;      // lane j keeps the j-th choice
   for (int j = 0; j < top; ++j) {
     unsigned long long best = keys[0];
-    int best_i = 0;
+    int best_i = at[0];
+    if constexpr (!SORTED) {
 #pragma unroll
-    for (int i = 1; i < PER; ++i)
-      if (keys[i] > best) {
-        best = keys[i];
-        best_i = i;
-      }
+      for (int i = 1; i < PER; ++i)
+        if (keys[i] > best) {
+          best = keys[i];
+          best_i = i;
+        }
+    }
     const uint32_t high = (uint32_t)(best >> 32), most = wave_largest(high);
     unsigned long long having = __ballot(high == most);
     if (having & (having - 1)) {      // several lanes: the lower halves decide, then the index
@@ -151,10 +180,18 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
       const uint32_t index = high == most && low == most_low ? (uint32_t)(lane + best_i * BH_WAVE) : 0xffffffffu;
       having = __ballot(index == over_wave(index, [](uint32_t a, uint32_t b) { return min(a, b); }) && high == most);
     }
-    const int winner = __builtin_amdgcn_readfirstlane(__ffsll(having) - 1), which = __builtin_amdgcn_readlane(best_i, winner);
+    const int winner = __builtin_ctzll(having), which = __builtin_amdgcn_readlane(best_i, winner);
+    if constexpr (SORTED) {
+      if (lane == winner) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (which == i && lane == winner) keys[i] = 0;
+        for (int i = 0; i + 1 < PER; ++i) keys[i] = keys[i + 1], at[i] = at[i + 1];
+        keys[PER - 1] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (which == i && lane == winner) keys[i] = 0;
+    }
     if (lane == j) mine_index = winner + which * BH_WAVE;
   }
   double mine = 0., sum = 0.;
@@ -163,8 +200,14 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_groups_kernel(const float
     const double theirs = __shfl(score[i], mine_index % BH_WAVE, BH_WAVE);
     if (mine_index / BH_WAVE == i) mine = theirs;
   }
-  if (renorm)
-    for (int j = 0; j < top; ++j) sum += of_lane(mine, j);
+  if (renorm) {      // (the first 32 lanes have choices)
+    sum = lane < top ? mine : 0.;
+    sum += turned<8>(sum);
+    sum += turned<4>(sum);
+    sum += turned<2>(sum);
+    sum += turned<1>(sum);
+    if (top > 16) sum += __shfl_xor(sum, 16, BH_WAVE);
+  }
   if (lane < top) {
     if (renorm) mine = sum == 0. ? 0. : mine / sum;
     chosen[(size_t)row * top + lane] = mine_index;
