@@ -352,51 +352,24 @@ void launch_few(const T* in, int in_div, const int32_t* chosen, int pairs, int E
 // A workgroup of 2 x 4 waves owns 32 XB pairs of one expert and 256 of its weight rows (gated: gate and up rows of the same 128 outputs), on
 // the ring of float8_ring.h with rows picked through the expert's list.  The gated form's 128 outputs are a stretch of the next product's
 // k: they are brought into 8 bits here, a pair's largest found between the four waves that hold its row.
+// XB is 4 from 48 pairs an expert on, where the last tile of an expert goes as one of 64 if it has no more (us, 128 experts of 2,048 x 768, as
+// tiles of 64 / so: 40 pairs each 194 / 208, 48 221 / 218, 62 238 / 233; 64 pairs each with whole last tiles 258, so 234, 128 each 348 / 336).
 // a: rows in 8 bits, row after row; the input of pair p is row p / in_div.  out: float32 [pairs][N]; gated: rows in 8 bits, row after row,
 // and their exponents, `out_padded` words a row of them.
 template <bool GATED, bool FULL, int XB>
-__global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded, int in_div,
-                                                              const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
-                                                              F8Weight w, void* __restrict__ out, uint8_t* __restrict__ out_exponents, int out_padded,
-                                                              ExpertGate gate, const float* __restrict__ in_weights) {
-  using Ring = F8Ring<FULL, XB, 4, 2, 4, 3, GATED ? 2 : 1, false, true>;
+using ExpertsRing = F8Ring<FULL, XB, 4, 2, 4, 3, GATED ? 2 : 1, false, true>;
+
+// The tile of pairs p0 .. and of weight rows tile_n.  (`ring` is not restrict: walk's own is, and within another the compiler has LDS reads wait for
+// the loads that are on their way to other places of the ring.)
+template <bool GATED, bool FULL, int XB>
+__device__ __forceinline__ void experts_ring_tile(f8_u32x4_t* ring, const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded,
+                                                  int in_div, const int32_t* __restrict__ pairs, int expert, int count, int p0, int tile_n, const F8Weight& w,
+                                                  void* __restrict__ out, uint8_t* __restrict__ out_exponents, int out_padded, const ExpertGate& gate,
+                                                  const float* __restrict__ in_weights) {
+  using Ring = ExpertsRing<GATED, FULL, XB>;
   constexpr int YB = Ring::YB, HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS, WN = Ring::WN;
-  __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[Ring::R * Ring::PIECES * 64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN;
-  const int N = w.rows, n_tiles = (N + OUTS - 1) / OUTS, steps = w.stretches, blocks = w.blocks();
-  // Tiles of pairs of all experts: a wave adds up 64 experts at a time; every wave of the workgroup finds the same.  Workgroups go to the
-  // eight XCDs in turn: every XCD takes a run of (expert, weight tile, tile of pairs) in this order.
-  int total = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) total += e0 + lane < E ? (counts[e0 + lane] + ROWS - 1) / ROWS : 0;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, BH_WAVE);
-  total *= n_tiles;
-  const int each = (total + 7) / 8, turn = blockIdx.x / 8, id = (blockIdx.x % 8) * each + turn;
-  if (turn >= each || id >= total) return;      // the whole workgroup
-  int expert = -1, before = 0, count = 0, at = 0;
-  for (int e0 = 0; e0 < E && expert < 0; e0 += 64) {
-    const int own = e0 + lane < E ? counts[e0 + lane] : 0, tiles = (own + ROWS - 1) / ROWS * n_tiles;
-    int upto = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int lower = __shfl_up(upto, off, BH_WAVE);
-      if (lane >= off) upto += lower;
-    }
-    const unsigned long long behind = __ballot(before + upto > id);
-    if (behind) {
-      const int l = __ffsll(behind) - 1;
-      expert = e0 + l;
-      count = __shfl(own, l, BH_WAVE);
-      at = id - before - (__shfl(upto, l, BH_WAVE) - __shfl(tiles, l, BH_WAVE));
-    } else {
-      before += __shfl(upto, 63, BH_WAVE);
-    }
-  }
-  expert = __builtin_amdgcn_readfirstlane(expert);
-  count = __builtin_amdgcn_readfirstlane(count);
-  at = __builtin_amdgcn_readfirstlane(at);
-  const int row_tiles = (count + ROWS - 1) / ROWS, p0 = (at % row_tiles) * ROWS, tile_n = at / row_tiles;
-  const int32_t* pairs = list + (size_t)expert * capacity;
+  const int N = w.rows, steps = w.stretches, blocks = w.blocks();
   const uint8_t* from[Ring::EACH];
   uint32_t row_at[Ring::ROW_PARTS];
 #pragma unroll
@@ -480,6 +453,54 @@ __global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __r
       }
     }
   }
+}
+
+template <bool GATED, bool FULL, int XB>
+__global__ __launch_bounds__(512, 2) void experts_ring_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, int padded, int in_div,
+                                                              const int32_t* __restrict__ list, int capacity, const int32_t* __restrict__ counts, int E,
+                                                              F8Weight w, void* __restrict__ out, uint8_t* __restrict__ out_exponents, int out_padded,
+                                                              ExpertGate gate, const float* __restrict__ in_weights) {
+  using Ring = ExpertsRing<GATED, FULL, XB>;
+  constexpr int ROWS = Ring::ROWS, OUTS = Ring::OUTS;
+  __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[Ring::R * Ring::PIECES * 64];
+  const int lane = threadIdx.x % 64, n_tiles = (w.rows + OUTS - 1) / OUTS;
+  // Tiles of pairs of all experts: a wave adds up 64 experts at a time; every wave of the workgroup finds the same.  Workgroups go to the
+  // eight XCDs in turn: every XCD takes a run of (expert, weight tile, tile of pairs) in this order.
+  int total = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) total += e0 + lane < E ? (counts[e0 + lane] + ROWS - 1) / ROWS : 0;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, BH_WAVE);
+  total *= n_tiles;
+  const int each = (total + 7) / 8, turn = blockIdx.x / 8, id = (blockIdx.x % 8) * each + turn;
+  if (turn >= each || id >= total) return;      // the whole workgroup
+  int expert = -1, before = 0, count = 0, at = 0;
+  for (int e0 = 0; e0 < E && expert < 0; e0 += 64) {
+    const int own = e0 + lane < E ? counts[e0 + lane] : 0, tiles = (own + ROWS - 1) / ROWS * n_tiles;
+    int upto = tiles;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int lower = __shfl_up(upto, off, BH_WAVE);
+      if (lane >= off) upto += lower;
+    }
+    const unsigned long long behind = __ballot(before + upto > id);
+    if (behind) {
+      const int l = __ffsll(behind) - 1;
+      expert = e0 + l;
+      count = __shfl(own, l, BH_WAVE);
+      at = id - before - (__shfl(upto, l, BH_WAVE) - __shfl(tiles, l, BH_WAVE));
+    } else {
+      before += __shfl(upto, 63, BH_WAVE);
+    }
+  }
+  expert = __builtin_amdgcn_readfirstlane(expert);
+  count = __builtin_amdgcn_readfirstlane(count);
+  at = __builtin_amdgcn_readfirstlane(at);
+  const int row_tiles = (count + ROWS - 1) / ROWS, p0 = (at % row_tiles) * ROWS, tile_n = at / row_tiles;
+  const int32_t* pairs = list + (size_t)expert * capacity;
+  if (XB == 4 && count - p0 <= 64)
+    experts_ring_tile<GATED, FULL, 2>(ring, a, exponents, padded, in_div, pairs, expert, count, p0, tile_n, w, out, out_exponents, out_padded, gate, in_weights);
+  else
+    experts_ring_tile<GATED, FULL, XB>(ring, a, exponents, padded, in_div, pairs, expert, count, p0, tile_n, w, out, out_exponents, out_padded, gate, in_weights);
 }
 
 // ---- the sum over a row's pairs --------------------------------------------------------------------------------
@@ -607,7 +628,7 @@ extern "C" int bh_experts_float8_tiles(const void* a, const void* exponents, int
   BH_REQUIRE((long)(rows + 15) * ((K + 511) / 512 * 512) < (1L << 32), "experts_float8: %d rows of %d inputs do not lie within 4 GB", rows, K);
   BH_REQUIRE(!gated || out_exponents != nullptr, "experts_float8: rows in 8 bits have exponents");
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
-  const bool wide = pairs >= 64L * E;      // tiles of 128 pairs
+  const bool wide = pairs >= 48L * E;
   const int outs = gated ? 128 : 256, tile = wide ? 128 : 64;
   const long most = (long)((N + outs - 1) / outs) * (pairs / tile + (pairs < E ? pairs : E)) + 8;      // every expert's last tile may be a part of one
   BH_REQUIRE(most < (1L << 31), "experts_float8: %d pairs of %d outputs are too many", pairs, N);
