@@ -1,6 +1,7 @@
 // Matrix products with weights and activations in 8 bits (float8.h): C[M, N] (+)= x[M, K] * W[N, K]^T, plain or gated.
-//   few     up to 16 rows straight from bfloat16 or float32 rows (a wave quantises the stretch it multiplies), up to 128 from rows in 8 bits
-//   rings   many rows (gemm_float8_ring.hip), K in parts where the tiles alone leave compute units idle, and their sum
+//   few     up to 16 rows straight from bfloat16 or float32 rows (a wave quantises the stretch it multiplies), up to 128 from rows in 8 bits where
+//           an estimate says so
+//   rings   more rows (gemm_float8_ring.hip), K in parts where the tiles alone leave compute units idle, and their sum
 #include "float8_few.h"
 #include "gemm_float8_ring.h"
 
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS = 16, FEW_ROWS_IN_8 = 128;
+constexpr int FEW_ROWS = 16, FEW_ROWS_ALWAYS = 48, FEW_ROWS_IN_8 = 128;      // `few`: the most rows as they are, in 8 bits always, and by an estimate
 
 int span_of(int N, int K, bool gated) {
   if (gated) return 16;
@@ -153,6 +154,30 @@ int span_of(int N, int K, bool gated) {
   if (2 * blocks <= units && K >= 1536) return 8;
   if (blocks > units && blocks < 2 * units && (N + 23) / 24 <= units) return 24;
   return 16;
+}
+
+// Blocks of 16 rows that the kernel for M rows is compiled for.
+int few_row_blocks(int M) { return M <= 32 ? 2 : M <= 48 ? 3 : M <= 64 ? 4 : M <= 96 ? 6 : 8; }
+
+// What `few` is estimated to take from rows in 8 bits (us): a start, and for a wave's every stretch the weights and the blocks of rows, which every
+// workgroup reads whole from the L2.  From the times that SHAPES of gemm_float8_ring.hip comes from (64 rows of 1,333 x 1,000 4.7, on the rings 6.4; 128 rows of 4,096 x
+// 4,096 12.1 and 10.6; 64 of 4,096 x 12,288 26.5 and 15.7).
+double few_cost_us(int M, int N, int K, bool gated, bool full) {
+  constexpr double STRETCH[2][3] = {{1.386, 1.800, 2.072}, {1.814, 2.243, 2.334}};      // of 4, 6 and 8 blocks of rows
+  const int span = span_of(N, K, gated), stretches = (K + F8_K - 1) / F8_K;
+  const double loads = (double)((N + span - 1) / span) * (gated ? 2. : span == 24 ? 1.5 : 1.) / bh_compute_units();
+  const double walk = (stretches + FEW_WAVES - 1) / FEW_WAVES * (loads > 1. ? loads : 1.) * STRETCH[full][few_row_blocks(M) / 2 - 2];
+  const double read = (double)(gated ? 2 : 1) * N * K / 4.47e6;
+  return 3.2 + (walk > read ? walk : read);
+}
+
+// Whether a product from rows in 8 bits goes through `few`; else the rings' plan.  Up to 48 rows it does: weights that come from memory, and not from the
+// caches as in the times behind the estimates, reach it sooner (steps of a model of 8 layers of 4,096 and 12,288, us, with the estimates alone / so: 32 rows 787 /
+// 772, 40 978 / 931, 48 967 / 928; the other way round from there on, 64 rows 1,064 by the estimates, 1,080 through `few`, 128 rows 1,409 and 1,500).
+bool few_takes(int M, int N, int K, bool gated, bool full, F8RingPlan* plan) {
+  if (M <= FEW_ROWS_ALWAYS) return true;
+  *plan = float8_ring_plan(M, N, K, gated, full);
+  return M <= FEW_ROWS_IN_8 && few_cost_us(M, N, K, gated, full) <= plan->us;
 }
 
 template <typename T, typename TC, bool GATED, bool FULL, int MB>
@@ -187,10 +212,11 @@ template <typename T, typename TC, bool GATED, bool FULL>
 void launch_few(const void* x, const uint32_t* exponents, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
 #define BH_F8_FEW(MB) launch_few_blocks<T, TC, GATED, FULL, MB>(x, exponents, w, c, M, K, ldc, accumulate, form, stream)
   if constexpr (sizeof(T) == 1) {
-    if (M <= 32) BH_F8_FEW(2);
-    else if (M <= 48) BH_F8_FEW(3);
-    else if (M <= 64) BH_F8_FEW(4);
-    else if (M <= 96) BH_F8_FEW(6);
+    const int row_blocks = few_row_blocks(M);
+    if (row_blocks <= 2) BH_F8_FEW(2);
+    else if (row_blocks == 3) BH_F8_FEW(3);
+    else if (row_blocks == 4) BH_F8_FEW(4);
+    else if (row_blocks == 6) BH_F8_FEW(6);
     else BH_F8_FEW(8);
   } else {
     BH_F8_FEW(1);
@@ -213,8 +239,8 @@ int fault_of(const void* w, const void* scales, const void* c, int c_dtype, int 
 extern "C" int bh_gemm_float8_few_rows() { return FEW_ROWS; }
 // Bytes of scratch memory of a product from rows in 8 bits.
 extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full) {
-  if (M <= FEW_ROWS_IN_8 || N <= 0 || K <= 0) return 0;
-  const F8RingPlan plan = float8_ring_plan(M, N, K, gated != 0, full != 0);
+  F8RingPlan plan;
+  if (M <= 0 || N <= 0 || K <= 0 || few_takes(M, N, K, gated != 0, full != 0, &plan)) return 0;
   return plan.parts > 1 ? (long)plan.parts * M * N * (gated ? 2 : 1) * 4 : 0;
 }
 
@@ -250,7 +276,8 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
   if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
   BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
   BH_REQUIRE((long)(M + 15) * ((K + 511) / 512) < (1L << 30), "gemm_float8: the exponents of %d rows of %d inputs do not lie within 4 GB", M, K);
-  if (M <= FEW_ROWS_IN_8) {
+  F8RingPlan plan;
+  if (few_takes(M, N, K, gate != 0, full != 0, &plan)) {
     const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
     const GateForm form = bh_gate_form(gate);
 #define BH_F8_RUN(TC, GATED, FULL) launch_few<uint8_t, TC, GATED, FULL>(a, (const uint32_t*)exponents, weight, (TC*)c, M, K, ldc, accumulate, form, stream)
@@ -258,7 +285,6 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
 #undef BH_F8_RUN
     return bh_check_launch("gemm_float8");
   }
-  const F8RingPlan plan = float8_ring_plan(M, N, K, gate != 0, full != 0);
   BH_REQUIRE(plan.parts == 1 || (scratch != nullptr && (uintptr_t)scratch % 16 == 0), "gemm_float8: a product in %d parts needs scratch memory", plan.parts);
   const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
   const GateForm form = bh_gate_form(gate);
@@ -272,4 +298,28 @@ extern "C" int bh_gemm_float8(const void* a, const void* exponents, const void* 
   } else if (gate) finish_kernel<bf16_t, true><<<grid, 256, 0, stream>>>((const float*)scratch, (bf16_t*)c, plan.parts, N, ldc, accumulate, form);
   else finish_kernel<bf16_t, false><<<grid, 256, 0, stream>>>((const float*)scratch, (bf16_t*)c, plan.parts, N, ldc, accumulate, form);
   return bh_check_launch("gemm_float8");
+}
+
+namespace {
+long rounded(long bytes) { return (bytes + 511) / 512 * 512; }
+long rows_bytes(int M, int K) { return rounded((M + 15L) / 16 * ((K + F8_K - 1) / F8_K) * F8_BLOCK); }
+long exponents_bytes(int M, int K) { return rounded((M + 15L) / 16 * 16 * ((K + 511) / 512) * 4); }
+}  // namespace
+
+// The same from rows as they are, through their 8 bits in `working`: so many bytes.
+extern "C" long bh_gemm_float8_working(int M, int N, int K, int gated, int full) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return rows_bytes(M, K) + exponents_bytes(M, K) + bh_gemm_float8_scratch(M, N, K, gated, full);
+}
+// x: null where `working` holds the rows in 8 bits already, from a product before with the same rows.
+extern "C" int bh_gemm_float8_rows(const void* x, int dtype, void* working, const void* w, const void* scales, void* c, int c_dtype, int accumulate, int M,
+                                   int N, int K, int ldc, int gate, int full, hipStream_t stream) {
+  if (const int fault = fault_of(w, scales, c, c_dtype, M, N, K, ldc, gate)) return fault;
+  BH_REQUIRE(working != nullptr && (uintptr_t)working % 16 == 0, "gemm_float8: rows in 8 bits need working memory");
+  uint8_t* data = (uint8_t*)working;
+  uint8_t* exponents = data + rows_bytes(M, K);
+  if (x != nullptr) {
+    if (const int status = float8_rows_launch(x, dtype, data, (uint32_t*)exponents, M, K, 0, 0, stream)) return status;
+  }
+  return bh_gemm_float8(data, exponents, w, scales, c, c_dtype, accumulate, M, N, K, ldc, gate, full, exponents + exponents_bytes(M, K), stream);
 }

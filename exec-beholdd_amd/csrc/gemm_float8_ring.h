@@ -2,9 +2,10 @@
 #pragma once
 #include "float8.h"
 
-// The tile that a product runs on (an index of SHAPES in gemm_float8_ring.hip), and in how many parts of K.
+// The tile that a product runs on (an index of SHAPES in gemm_float8_ring.hip), in how many parts of K, and what that is estimated to take.
 struct F8RingPlan {
   int tile, parts;
+  double us;
 };
 F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full);
 // a, exponents: rows in 8 bits, in blocks.  c: [M] rows of `ldc` elements; gated: w holds two matrices.  In more than one part the bare sums are

@@ -106,37 +106,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
   }
 }
 
-// A tile's sizes, how many of its workgroups share a compute unit, what a step of 128 k costs a compute unit that has one of them, or two, and what
-// their start and end cost, with the matrix cores' own sums and with full ones (us).  From the times of every tile and cut of K for 9 products of 129
-// to 8,160 rows, 1,024 to 24,576 weight rows and k of 1,000 to 12,288 (94 sizes, 1,300 times): what this chooses there takes 1 % longer than the best
-// of them on average, 11 % at most.  Where the tiles are ahead, us, 64 x 256 / 128 x 128 / 256 x 128 / 256 x 256: 512 rows of 4,096 x 4,096 21.1 / 28.7 /
-// 33 / 55; 2,048 rows 45.3 / 39.6 / 41.5 / 57; 4,096 rows 88 / 75.6 / 81.4 / 69.8; 200 rows of 12,288 k in four parts 26.3, in one 55.
+// A tile's sizes, how many of its workgroups share a compute unit, what a step of 128 k costs a compute unit that has one of them, two or three, and
+// what their start and end cost, with the matrix cores' own sums and with full ones (us).  From the times of every tile and cut of K, and of few rows
+// (gemm_float8.hip), for 12 products of 24 to 8,160 rows, 1,024 to 24,576 weight rows and k of 1,000 to 12,288 (220 sizes, 3,500 times): what is chosen there
+// takes 2 % longer than the best of them on average, 22 % at most (300 rows of 1,024 x 1,024 7.0 / 5.8).  Where the tiles are ahead, us, 32 x 64 / 64 x 64 /
+// 64 x 256 / 128 x 128 / 256 x 128 / 256 x 256: 256 rows of 2,048 x 2,048 6.4 / 7.9 / 13.6 / 16.3 / 18.1 / 24; 512 rows of 4,096 x 4,096 18.2 / 17.6 / 20.7 / 28.7 / 33 / 55; 2,048 rows of them
+// from the third on 45.3 / 39.6 / 41.5 / 57, 4,096 rows 88 / 75.6 / 81.4 / 69.8; 200 rows of 4,096 x 12,288 in four parts of 64 x 256 26.3, in one 55.
 struct TileShape {
   int rows, columns, share;
-  double step, step_shared, start_and_end, full_step, full_step_shared, full_start_and_end;
+  double step[3], start_and_end, full_step[3], full_start_and_end;
 };
-constexpr TileShape SHAPES[] = {{128, 128, 2, 0.755, 1.122, 3.5, 1.163, 1.637, 6.8},
-                                {256, 128, 1, 0.861, 0., 6.3, 1.545, 0., 9.5},
-                                {256, 256, 1, 1.489, 0., 9.8, 0., 0., 0.},
-                                {64, 256, 1, 0.561, 0., 4.3, 0.944, 0., 5.4},
-                                {128, 256, 1, 0.863, 0., 6.4, 1.555, 0., 9.2}};
-constexpr int TILES = 5, MOST_PARTS = 8;
+constexpr TileShape SHAPES[] = {{128, 128, 2, {0.738, 1.101}, 3.94, {1.145, 1.761}, 6.24},
+                                {256, 128, 1, {0.798}, 6.74, {1.610}, 8.36},
+                                {256, 256, 1, {1.392}, 10.37, {}, 0.},
+                                {64, 256, 1, {0.516}, 4.79, {0.959}, 5.50},
+                                {128, 256, 1, {0.811}, 6.74, {1.577}, 8.99},
+                                {64, 64, 3, {0.287, 0.432, 0.574}, 3.25, {0.462, 0.780, 0.860}, 3.78},
+                                {32, 64, 3, {0.212, 0.294, 0.385}, 3.19, {0.334, 0.495, 0.557}, 3.55}};
+constexpr int TILES = 7, MOST_PARTS = 8;
 
 double cost_us(int tile, int parts, int M, int W, int K, bool full) {
   const TileShape& s = SHAPES[tile];
   const long units = bh_compute_units(), workgroups = (long)((M + s.rows - 1) / s.rows) * ((W + s.columns - 1) / s.columns) * parts;
-  const double steps = ((K + F8_K - 1) / F8_K + parts - 1) / parts;
-  const double ends = full ? s.full_start_and_end : s.start_and_end;
-  const double alone = steps * (full ? s.full_step : s.step) + ends, both = steps * (full ? s.full_step_shared : s.step_shared) + ends;
-  double t;
-  if (s.share == 1) {
-    t = (double)((workgroups + units - 1) / units) * alone;
-  } else {      // whole rounds of two a compute unit, then a last one: of two, which take as long on some units as on all, or of one
-    const long rest = workgroups % (2 * units);
-    t = (double)(workgroups / (2 * units)) * both + (rest > units ? both : rest > 0 ? alone : 0.);
-  }
+  const double steps = ((K + F8_K - 1) / F8_K + parts - 1) / parts, ends = full ? s.full_start_and_end : s.start_and_end;
+  const double* step = full ? s.full_step : s.step;
+  // whole rounds of `share` a compute unit, then a last one of as many as are left, which take as long on some units as on all
+  const long rounds = workgroups / (units * s.share), left = (workgroups % (units * s.share) + units - 1) / units;
+  double t = rounds * (steps * step[s.share - 1] + ends);
+  if (left > 0) t += steps * step[left - 1] + ends;
+  const double read = ends + (double)W * K / 4.47e6;      // no sooner than the weights are there
+  if (t < read) t = read;
   if (parts == 1) return t;
-  return t + 4.0 + parts * (double)M * W * 8.0 / 7.3e6;      // the parts' sums on their way to memory and back, and a launch
+  return t + 2.7 + parts * (0.113 + (double)M * W * 8. / 7.42e6);      // the parts' sums on their way to memory and back, and a launch
 }
 
 template <typename TC, bool GATED, bool FULL, bool PARTS>
@@ -151,6 +152,8 @@ void launch(int tile, int parts, const uint8_t* a, const uint32_t* exponents, co
   else if (tile == 1) BH_F8_RING(FULL, 4, 4, 4, 2, 3, false, 8, 4);
   else if (tile == 3) BH_F8_RING(FULL, 2, 4, 2, 4, 3, false, 8, 4);
   else if (tile == 4) BH_F8_RING(FULL, 4, 4, 2, 4, 3, false, 8, 4);
+  else if (tile == 5) BH_F8_RING(FULL, 2, 2, 2, 2, 3, false, 8, 8);
+  else if (tile == 6) BH_F8_RING(FULL, 1, 2, 2, 2, 4, false, 8, 8);
   else if constexpr (!FULL && !PARTS) BH_F8_RING(false, 4, 8, 4, 2, 3, true, 8, 4);
 #undef BH_F8_RING
 }
@@ -165,8 +168,7 @@ void launch_plan(const F8RingPlan& plan, const uint8_t* a, const uint32_t* expon
 }  // namespace
 
 F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full) {
-  F8RingPlan plan = {0, 1};
-  double least = 0.;
+  F8RingPlan plan = {0, 1, 0.};
   const int W = gated ? 2 * N : N, stretches = (K + F8_K - 1) / F8_K;
   for (int tile = 0; tile < TILES; ++tile) {
     if (tile == 2 && full) continue;      // (full sums have no registers for it)
@@ -174,7 +176,7 @@ F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full) {
     const int most = tile == 2 || M > 65535 || tiles >= 2L * bh_compute_units() ? 1 : MOST_PARTS;
     for (int parts = 1; parts <= most && (parts == 1 || stretches >= 4 * parts); ++parts) {
       const double cost = cost_us(tile, parts, M, W, K, full);
-      if (least == 0. || cost < least) least = cost, plan = {tile, parts};
+      if (plan.us == 0. || cost < plan.us) plan = {tile, parts, cost};
     }
   }
   return plan;

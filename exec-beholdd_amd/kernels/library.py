@@ -193,6 +193,7 @@ class KernelSizes:
         except OSError as error:
             raise KernelError(f"cannot load the HIP kernel library {path}: {error}") from None
         self.library_path = path
+        self._float8_most: dict = {}      # (m, n, k, gated) -> the most scratch bytes of a product of up to m rows
         self._declare()
 
     # ---- ctypes declarations ----
@@ -312,6 +313,7 @@ class KernelSizes:
             "bh_gemm_float8_few_rows": [],
             "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
+            "bh_gemm_float8_rows": [p, i, p, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
             "bh_experts_float8_few": [i, i],
             "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
@@ -325,6 +327,7 @@ class KernelSizes:
             function.argtypes = argtypes
             function.restype = i
         lib.bh_gemm_float8_scratch.argtypes, lib.bh_gemm_float8_scratch.restype = [i, i, i, i, i], ctypes.c_long
+        lib.bh_gemm_float8_working.argtypes, lib.bh_gemm_float8_working.restype = [i, i, i, i, i], ctypes.c_long
         lib.bh_gemm_bf16_scratch.argtypes = [i, i, i, i, i]
         lib.bh_gemm_bf16_scratch.restype = ctypes.c_long
         for query, count in ((lib.bh_lightning_products_scratch, 10), (lib.bh_ssm_products_scratch, 8), (lib.bh_lightning_products_most, 6),
@@ -369,10 +372,16 @@ class KernelSizes:
     def gemm_float8_working_bytes(self, m, n, k, act_size, gated=False) -> int:
         """Bytes that a product with an 8-bit weight allocates beside its output (n rows of one of the weight's matrices): the rows in plain
         order where they come in blocks, the rows in 8 bits, and the sums of K in parts."""
-        m, n, k = int(m), int(n), int(k)
+        m, n, k, gated = int(m), int(n), int(k), int(bool(gated))
         total = _rounded(m * k * act_size)
-        if m > int(self.lib.bh_gemm_float8_few_rows()):
-            scratch = max(int(self.lib.bh_gemm_float8_scratch(m, n, k, int(bool(gated)), full)) for full in (0, 1))
+        few = int(self.lib.bh_gemm_float8_few_rows())
+        if m > few:
+            key = (m, n, k, gated)
+            scratch = self._float8_most.get(key)
+            if scratch is None:      # fewer rows may be cut into more parts; within 16 rows the number of parts does not grow with them
+                answer = self.lib.bh_gemm_float8_scratch
+                scratch = self._float8_most[key] = max(int(answer(rows, n, k, gated, full)) // rows * min(rows + 15, m)
+                                                       for rows in range(few + 1, m + 1, 16) for full in (0, 1))
             total += sum(_rounded(size) for size in Float8Rows.bytes_of(m, k)) + _rounded(scratch)
         return total
 
@@ -476,7 +485,7 @@ class HipKernels(KernelSizes):
         self._squares: dict = {}    # (m, n, k) -> which product squares its output (`gemm_relu_squared`), or 0
         self._clamps: dict = {}     # (m, n, k) -> which gated product clamps (`gemm_clamped_glu`), or 0
         self._bare: dict = {}       # (m, n, k) -> the parts that `gemm_bare` leaves such a product in, or 0
-        self._float8_scratch: dict = {}      # (m, n, k, gated, full sums) -> scratch bytes of a product from rows in 8 bits
+        self._float8_working: dict = {}      # (rows in 8 bits already, m, n, k, gated, full sums) -> bytes that a product takes beside its output
         self._float8_experts: dict = {}      # (pairs, experts, top) -> whether they are one row's, and whether the kernels of few pairs take them
         self._float8_few_rows = int(self.lib.bh_gemm_float8_few_rows())      # up to so many rows a product takes them as they are
         self.page_size = int(self.lib.bh_page_size())
@@ -1016,35 +1025,35 @@ class HipKernels(KernelSizes):
             raise KernelError("gemm: a product with an 8-bit weight writes plain rows")
         if w.device != self.device or a.device != self.device:
             raise KernelError(f"gemm: rows on {a.device} and a weight on {w.device}, expected {self.device}")
-        few = type(a) is torch.Tensor and m <= self._float8_few_rows
-        if not few:
-            if not isinstance(a, Float8Rows):
-                a = self._plain_rows(a)
-                few = m <= self._float8_few_rows
-                if not few:
-                    a = self.to_float8(a)
-            elif a.in_rows:
-                raise KernelError("gemm: rows in 8 bits go into a product in blocks")
+        ready = isinstance(a, Float8Rows)
+        if ready and a.in_rows:
+            raise KernelError("gemm: rows in 8 bits go into a product in blocks")
+        if type(a) is not torch.Tensor and not ready:
+            a = self._plain_rows(a)
         out_at, c_code, stream, accumulate = self._ptr(out, "gemm out"), _code(out, "gemm out"), self._stream(), int(bool(accumulate))
         data, scales = w.data.data_ptr(), w.scales.data_ptr()
-        if few:
-            a_at, a_code = self._ptr(a, "gemm a"), _code(a, "gemm a")
-        else:
-            key = (m, n, k, gate != 0, full)
-            scratch_bytes = self._float8_scratch.get(key)
-            if scratch_bytes is None:
-                scratch_bytes = self._float8_scratch[key] = int(self.lib.bh_gemm_float8_scratch(*map(int, key)))
-            scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=self.device) if scratch_bytes else None
-            a_at, exponents, scratch_at = a.data.data_ptr(), a.exponents.data_ptr(), scratch.data_ptr() if scratch is not None else None
+        a_at, a_code = (a.data.data_ptr(), 0) if ready else (self._ptr(a, "gemm a"), _code(a, "gemm a"))
+        few = not ready and m <= self._float8_few_rows
+        if not few:      # memory beside the output: the sums of K in parts, and, if they are still to be made, the rows in 8 bits
+            key = (ready, m, n, k, gate != 0, full)
+            working_bytes = self._float8_working.get(key)
+            if working_bytes is None:
+                answer = self.lib.bh_gemm_float8_scratch if ready else self.lib.bh_gemm_float8_working
+                working_bytes = self._float8_working[key] = int(answer(*map(int, key[1:])))
+            working = torch.empty(working_bytes, dtype=torch.uint8, device=self.device) if working_bytes else None
+            working_at = working.data_ptr() if working is not None else None
         for i in range(matrices):
             if i:
                 data, out_at = data + Float8Weight.data_bytes(1, n, k), out_at + n * out.element_size()
                 scales += 4 * w.scales.shape[1] * w.scales.shape[2]
             if few:
                 self._check(self.lib.bh_gemm_float8_few(a_at, a_code, data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1], gate, full, stream))
-            else:
-                self._check(self.lib.bh_gemm_float8(a_at, exponents, data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1], gate, full, scratch_at,
-                                                    stream))
+            elif ready:
+                self._check(self.lib.bh_gemm_float8(a_at, a.exponents.data_ptr(), data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1], gate, full,
+                                                    working_at, stream))
+            else:      # (the rows stay for the matrices after the first)
+                self._check(self.lib.bh_gemm_float8_rows(None if i else a_at, a_code, working_at, data, scales, out_at, c_code, accumulate, m, n, k, out.shape[1],
+                                                         gate, full, stream))
 
     def experts_float8(self, x, chosen, weights, w_up, w_down, out, limit=float("inf"), alpha=1.0, shift=0.0, weigh_input=False, fresh=False, through=None,
                        full_sums=None):

@@ -348,6 +348,29 @@ def test_tiles_and_parts_of_k(k, m, n, width, full):
     assert bool(torch.isfinite(out).all())
 
 
+@pytest.mark.parametrize("m,n,width,full,gated", [
+    (20, 130, 640, False, False), (20, 130, 640, True, True), (48, 130, 384, True, False), (60, 130, 384, False, False), (60, 100, 384, True, True),
+    (90, 130, 384, False, False), (90, 130, 384, True, True), (128, 130, 384, True, False), (100, 2050, 640, False, False), (100, 130, 3000, False, False),
+    (50, 300, 5000, True, False), (129, 64, 130, False, True), (129, 64, 3000, True, True), (129, 64, 3000, False, False), (5000, 300, 130, False, False),
+    (2600, 300, 130, True, True), (400, 512, 4200, False, False), (2100, 100, 3000, True, True), (1000, 2050, 4200, False, False), (400, 4100, 130, False, True),
+    (2600, 300, 4200, True, True), (2100, 2050, 3000, True, False), (1000, 2050, 3000, True, True), (1000, 4100, 130, False, False), (1000, 2050, 130, True, True),
+    (1000, 4100, 1500, False, False), (1000, 2050, 1500, False, True), (5000, 1030, 2048, True, False), (2100, 4100, 1000, False, False), (1000, 4100, 1000, False, True)])
+def test_every_kernel_of_products_from_rows_in_8_bits(k, m, n, width, full, gated):
+    """Few rows in every number of blocks, every tile of the rings, K whole and in parts, plain and gated: some rows of each."""
+    matrices = 2 if gated else 1
+    x, (w, held) = _rows(m, width, torch.bfloat16, 1), _weight(k, matrices, n, width, 2)
+    out = torch.full((m, n), math.nan, device=DEVICE)
+    (k.gemm_swiglu if gated else k.gemm)(x.to(DEVICE), w, out, full_sums=full)
+    pick = sorted({0, 1, 15, 16, 31 % m, 32 % m, 63 % m, 64 % m, 127 % m, 128 % m, m // 2, m - 2, m - 1})
+    x8, whole = plain.rows(x[pick]), plain.matrix(*held)
+    if gated:
+        want, bound = plain.gated(*plain.product(x8, whole[:n], full), *plain.product(x8, whole[n:], full))
+    else:
+        want, bound = plain.product(x8, whole, full)
+    _close(out[pick], want, bound)
+    assert bool(torch.isfinite(out).all())
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 def test_refusals(k):
