@@ -147,6 +147,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
 
 // ---- which kernel ----------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS = 16, FEW_ROWS_ALWAYS = 48, FEW_ROWS_IN_8 = 128;      // `few`: the most rows as they are, in 8 bits always, and by an estimate
+// (Steps of a model of 8 layers of 4,096 and 12,288 with rows as they are / in 8 bits, us: 17 sequences 791 / 732, 32 970 / 772: every workgroup quantises all rows.)
 
 int span_of(int N, int K, bool gated) {
   if (gated) return 16;

@@ -310,6 +310,8 @@ class KernelSizes:
             "bh_weighted_sum": [p, p, f, p, f, ctypes.c_long, p],
             "bh_experts_combine": [p, p, p, p, p, i, p, i, i, i, i, i, p],
             "bh_float8_rows": [p, i, p, p, i, i, i, i, p],
+            "bh_float8_norm_columns": [],
+            "bh_float8_norm": [p, p, i, f, i, p, p, i, i, p],
             "bh_gemm_float8_few_rows": [],
             "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
@@ -487,6 +489,7 @@ class HipKernels(KernelSizes):
         self._bare: dict = {}       # (m, n, k) -> the parts that `gemm_bare` leaves such a product in, or 0
         self._float8_working: dict = {}      # (rows in 8 bits already, m, n, k, gated, full sums) -> bytes that a product takes beside its output
         self._float8_experts: dict = {}      # (pairs, experts, top) -> whether they are one row's, and whether the kernels of few pairs take them
+        self._float8_norm_columns = int(self.lib.bh_float8_norm_columns())
         self._float8_few_rows = int(self.lib.bh_gemm_float8_few_rows())      # up to so many rows a product takes them as they are
         self.page_size = int(self.lib.bh_page_size())
         if self.page_size != _build.source_page_size():
@@ -996,6 +999,23 @@ class HipKernels(KernelSizes):
         out = self._new_float8_rows(rows, width, in_rows)
         self._check(self.lib.bh_float8_rows(self._ptr(x, "rows"), _code(x, "rows"), out.data.data_ptr(), out.exponents.data_ptr(), rows, width,
                                             int(out.in_rows), self.GATES[gate] if gate else 0, self._stream()))
+        return out
+
+    def rmsnorm_float8(self, x, weight, eps, dtype=torch.float32) -> Float8Rows | None:
+        """What `rmsnorm` would write as `dtype` (x float32 [n, D], weight [D] or None), as `Float8Rows`, for products with a `Float8Weight` that
+        alone read them; None where such a product takes rows as they are, or the rows are wider than the kernel takes (then call
+        `rmsnorm`)."""
+        if x.dim() != 2 or (weight is not None and weight.shape != (x.shape[1],)):
+            raise KernelError(f"rmsnorm_float8: rows {tuple(x.shape)} and weight {tuple(weight.shape) if weight is not None else None} do not fit")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"rmsnorm_float8: rows of float32 or bfloat16, got {dtype}")
+        rows, width = x.shape
+        if rows <= self._float8_few_rows or width > self._float8_norm_columns:
+            return None
+        out = self._new_float8_rows(rows, width, False)
+        self._check(self.lib.bh_float8_norm(self._ptr(x, "rmsnorm x", (torch.float32,)), self._ptr(weight, "rmsnorm weight", None, True),
+                                            _code(weight, "rmsnorm weight") if weight is not None else F32, float(eps), int(dtype == torch.bfloat16),
+                                            out.data.data_ptr(), out.exponents.data_ptr(), rows, width, self._stream()))
         return out
 
     def from_float8(self, x) -> torch.Tensor:

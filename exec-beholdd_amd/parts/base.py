@@ -199,10 +199,11 @@ class StepSize:
 class ProductReader:
     """The matrix product that reads an activation matrix next: `outputs` columns of result, through the
     gated activation or not (then its weight has twice as many rows); `packed`: its weight is in the kernel
-    library's own form (`Linear.prepare`), not a plain matrix."""
+    library's own form (`Linear.prepare`), not a plain matrix; `float8`: in 8 bits, so that it reads rows in 8 bits."""
     outputs: int
     swiglu: bool = False
     packed: bool = True
+    float8: bool = False
 
 
 @dataclass

@@ -65,7 +65,8 @@ class Linear:
     def reader(self, swiglu: bool = False) -> ProductReader:
         """This map as the only reader of an activation matrix (`swiglu`: its rows are gate rows, then up rows)."""
         return ProductReader(self.out_features // 2 if swiglu else self.out_features, swiglu,
-                             packed=self.weight is not None and not isinstance(self.weight, torch.Tensor) and not self.float8)
+                             packed=self.weight is not None and not isinstance(self.weight, torch.Tensor) and not self.float8,
+                             float8=bool(self.float8) and not self.shared)
 
     def packs(self, act_size: int) -> bool:
         """Whether `prepare` regroups this matrix in an engine of that element size."""

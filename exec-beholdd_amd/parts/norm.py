@@ -31,6 +31,10 @@ class RMSNorm:
     serves_reader = True   # forward and request take the product that reads the output
 
     def forward(self, ctx, hidden, rows=None, reader=None):
+        in_float8 = getattr(ctx.kernels, "rmsnorm_float8", None) if rows is None and getattr(reader, "float8", False) else None
+        out = in_float8(hidden, self.weight, self.eps, ctx.act_dtype) if in_float8 is not None else None
+        if out is not None:
+            return out
         n = hidden.shape[0] if rows is None else rows.shape[0]
         out = ctx.new_activations(n, self.width, reader=reader)
         ctx.kernels.rmsnorm(hidden, self.weight, self.eps, out, rows=rows)

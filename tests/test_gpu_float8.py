@@ -92,6 +92,42 @@ def test_gated_rows_in_8_bits(k, gate, dtype, n, width):
     assert (got != held).double().mean() < 0.01      # only what lies next to a border may fall on its other side
 
 
+@pytest.mark.parametrize("weight_dtype", [torch.float32, torch.bfloat16, None])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,width", [(17, 1), (33, 70), (40, 512), (130, 1001), (300, 4096), (18, 8192)])
+def test_normed_rows_in_8_bits(k, weight_dtype, dtype, n, width):
+    """float32 sums of squares of up to 8192 values in 8 + 6 + 16 roundings, half of their 2^-24 each in the root, and five more: 20 * 2^-24 of a value.
+    Rounded to bfloat16 on the way, that may give its neighbour, 2^-7 of it away."""
+    x = _rows(n, width, torch.float32, 5) * 3.0
+    x[1] = 0.0
+    weight = None if weight_dtype is None else (torch.randn(width, generator=torch.Generator().manual_seed(2)) + 1.0).to(weight_dtype)
+    value = x.double() / torch.sqrt((x.double() ** 2).mean(dim=1, keepdim=True) + 1e-5) * (1.0 if weight is None else weight.double())
+    on_device = x.to(DEVICE), None if weight is None else weight.to(DEVICE), 1e-5
+    rows = k.rmsnorm_float8(*on_device, dtype)
+    got = k.from_float8(rows).double().cpu()
+    if dtype == torch.bfloat16:      # the same bytes as from the rounded norm, but for a sum of squares in another order
+        rounded = torch.empty((n, width), dtype=dtype, device=DEVICE)
+        k.rmsnorm(*on_device, rounded)
+        value = rounded.double().cpu()
+    held, off = plain.requantised(value, value.abs() * (2.0 ** -19 if dtype == torch.float32 else 2.0 ** -7) + 1e-37)
+    assert bool(((got - held).abs() <= off).all())
+    assert (got != held).double().mean() < 0.01      # only what lies next to a border may fall on its other side
+    w, matrix = _weight(k, 1, 50, width, 3)
+    out = torch.empty((n, 50), device=DEVICE)
+    k.gemm(rows, w, out)
+    _close(out, *plain.product(got, plain.matrix(*matrix), True))
+
+
+def test_normed_rows_where_the_kernel_has_none(k):
+    from beholdd.kernels.library import KernelError
+    assert k.rmsnorm_float8(torch.ones((16, 64), device=DEVICE), None, 1e-5) is None
+    assert k.rmsnorm_float8(torch.ones((17, 8200), device=DEVICE), None, 1e-5) is None
+    for x, weight in ((torch.ones((20, 64), device=DEVICE, dtype=torch.bfloat16), None), (torch.ones((20, 64), device=DEVICE), torch.ones(63, device=DEVICE)),
+                      (torch.ones(64, device=DEVICE), None), (torch.ones((20, 128), device=DEVICE)[:, ::2], None)):
+        with pytest.raises(KernelError):
+            k.rmsnorm_float8(x, weight, 1e-5)
+
+
 @pytest.mark.parametrize("matrices,n,width", [(1, 1, 1), (1, 130, 257), (2, 24, 128), (3, 144, 300)])
 def test_weights_in_8_bits(k, matrices, n, width):
     w, held = _weight(k, matrices, n, width, 3)
