@@ -324,3 +324,22 @@ extern "C" int bh_gemm_float8_rows(const void* x, int dtype, void* working, cons
   }
   return bh_gemm_float8(data, exponents, w, scales, c, c_dtype, accumulate, M, N, K, ldc, gate, full, exponents + exponents_bytes(M, K), stream);
 }
+
+// Whether a gated product leaves its outputs in 8 bits itself: where its tiles take no longer than others and what would bring the outputs into 8 bits then, a
+// launch and a pass over the outputs (so / in two, us, 2 x 12,288 x 4,096: 128 rows 23.9 / 27.3, 512 57.6 / 60.2, 2,048 185 / 201, 8,192 756 / 801; fewer rows are
+// faster in two when weights come from memory, steps of 64 sequences of 8 such layers 1,068 / 1,019).
+extern "C" int bh_gemm_float8_gives_8(int M, int N, int K, int full) {
+  if (M < FEW_ROWS_IN_8 || N <= 0 || K <= 0) return 0;
+  return float8_ring_plan(M, N, K, true, full != 0, true).us <= float8_ring_plan(M, N, K, true, full != 0).us + 2.5 + (double)M * N / 2.2e6;
+}
+// A gated product from rows in 8 bits to rows in 8 bits, both in blocks: N outputs, of matrices of N gate and N up rows.
+extern "C" int bh_gemm_float8_gated_to_8(const void* a, const void* exponents, const void* w, const void* scales, void* c, void* c_exponents, int through_bf16,
+                                         int M, int N, int K, int gate, int full, hipStream_t stream) {
+  if (const int fault = fault_of(w, scales, c, BH_F32, M, N, K, N, gate)) return fault;
+  BH_REQUIRE(gate != 0 && M >= FEW_ROWS_IN_8, "gemm_float8: gated products of %d rows or more give rows in 8 bits", FEW_ROWS_IN_8);
+  BH_REQUIRE(((uintptr_t)a | (uintptr_t)exponents | (uintptr_t)c | (uintptr_t)c_exponents) % 16 == 0, "gemm_float8: the rows must be 16-byte aligned");
+  BH_REQUIRE((long)(M + 15) * ((K + 511) / 512) < (1L << 30), "gemm_float8: the exponents of %d rows of %d inputs do not lie within 4 GB", M, K);
+  const F8Weight weight = {(const uint8_t*)w, (const float*)scales, N, (K + F8_K - 1) / F8_K};
+  return float8_ring_launch_in_8(float8_ring_plan(M, N, K, true, full != 0, true), (const uint8_t*)a, (const uint32_t*)exponents, weight, (uint8_t*)c,
+                                 (uint8_t*)c_exponents, through_bf16, M, full, bh_gate_form(gate), stream);
+}

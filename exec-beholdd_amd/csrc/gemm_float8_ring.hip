@@ -28,11 +28,57 @@ __device__ inline void tile_of_workgroup(int n_tiles, int m_tiles, int* tile_n, 
   *tile_n = first_n + within / rows;
 }
 
+// The gated outputs of a tile, a stretch of the next product's k, in 8 bits, in blocks and with their exponents: a row's largest is found between the
+// waves that hold it.  `through_bf16`: they are rounded to bfloat16 first, as they would be on their way there.
+template <typename Ring>
+__device__ inline void leave_in_8(f8_u32x4_t* ring, f8_f32x4_t (&acc)[Ring::XB][Ring::YB], int tile_m, int tile_n, uint8_t* __restrict__ c,
+                                  uint8_t* __restrict__ c_exponents, int M, int N, int through_bf16, const GateForm& form) {
+  constexpr int XB = Ring::XB, HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS, WN = Ring::WN;
+  static_assert(Ring::G == 2 && OUTS == F8_K, "a tile's outputs are a stretch");
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wm = wave / WN, wn = wave % WN, padded = (M + 15) / 16 * 16;
+  uint32_t* largest = reinterpret_cast<uint32_t*>(ring);      // [wave column][row]
+  __syncthreads();      // every wave has read its last step
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int y = 0; y < HALF; ++y)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = tile_n * OUTS + (wn * HALF + y) * 16 + 4 * (lane / 16) + e;
+        float v = n < N ? f8_gate_mul(acc[x][y][e], acc[x][y + HALF][e], form) : 0.f;
+        if (through_bf16) v = to_f32(from_f32<bf16_t>(v));
+        acc[x][y][e] = v;
+        most = f8_larger(most, v);
+      }
+    most = f8_largest_of_row(most);
+    if (lane < 16) largest[wn * ROWS + (wm * XB + x) * 16 + lane] = most;
+  }
+  __syncthreads();
+  const int out_stretches = (N + F8_K - 1) / F8_K;
+#pragma unroll
+  for (int x = 0; x < XB; ++x) {
+    const int r = (wm * XB + x) * 16 + lane % 16, row = tile_m * ROWS + r;
+    uint32_t most = largest[r];
+#pragma unroll
+    for (int column = 1; column < WN; ++column) most = max(most, largest[column * ROWS + r]);
+    const uint32_t exponent = f8_exponent(most);
+    if (row >= M) continue;
+    uint8_t* block = c + ((size_t)(row / 16) * out_stretches + tile_n) * F8_BLOCK;
+#pragma unroll
+    for (int y = 0; y < HALF; ++y)
+      *reinterpret_cast<uint32_t*>(block + f8_place(row % 16, (wn * HALF + y) * 16 + 4 * (lane / 16))) =
+          f8_four(acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3], f8_scale(exponent));
+    if (wn == 0 && lane < 16) c_exponents[((size_t)(tile_n / 4) * padded + row) * 4 + tile_n % 4] = (uint8_t)exponent;
+  }
+}
+
 // A tile that sticks out of the matrix repeats its last blocks and stores only what exists.
 // With K in parts (PARTS, grid y) part p leaves its bare sums at c + p * M * width, width = N, or 2 N of a gated product (gate, then up).
+// TC uint8_t: a gated product of 128 outputs a tile leaves them in 8 bits (leave_in_8; `accumulate` is its `through_bf16`).
 template <typename TC, bool GATED, bool FULL, bool PARTS, int XB, int YB, int WM, int WN, int R, bool DIRECT, int BM, int BN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint8_t* __restrict__ a, const uint32_t* __restrict__ exponents, F8Weight w,
-                                                                     TC* __restrict__ c, int M, int ldc, int accumulate, GateForm form) {
+                                                                     TC* __restrict__ c, uint8_t* __restrict__ c_exponents, int M, int ldc, int accumulate, GateForm form) {
   using Ring = F8Ring<FULL, XB, YB, WM, WN, R, GATED ? 2 : 1, DIRECT>;
   constexpr int HALF = Ring::HALF, ROWS = Ring::ROWS, OUTS = Ring::OUTS;
   __shared__ __attribute__((aligned(16))) f8_u32x4_t ring[R * Ring::PIECES * 64];      // [step in turn][A's pieces, then W's][lane]
@@ -66,41 +112,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
   f8_f32x4_t acc[XB][YB];
   Ring::walk(ring, from, row_at, F8_BLOCK, exponents, x_at, padded, ws, first, steps, acc);
 
-  const bool fours = (N | ldc) % 4 == 0 && (uintptr_t)c % (4 * sizeof(TC)) == 0;
+  if constexpr (sizeof(TC) == 1) {
+    leave_in_8<Ring>(ring, acc, tile_m, tile_n, c, c_exponents, M, N, accumulate, form);
+  } else {
+    const bool fours = (N | ldc) % 4 == 0 && (uintptr_t)c % (4 * sizeof(TC)) == 0;
 #pragma unroll
-  for (int x = 0; x < XB; ++x) {
-    const int row = tile_m * ROWS + (wm * XB + x) * 16 + lane % 16;
-    if (row >= M) continue;
+    for (int x = 0; x < XB; ++x) {
+      const int row = tile_m * ROWS + (wm * XB + x) * 16 + lane % 16;
+      if (row >= M) continue;
 #pragma unroll
-    for (int y = 0; y < (PARTS ? YB : HALF); ++y) {
-      const int n = ((tile_n * WN + wn) * HALF + y % HALF) * 16 + 4 * (lane / 16);
-      if (n >= N) continue;
-      if constexpr (PARTS) {
-        const size_t width = GATED ? 2 * (size_t)N : N;
-        float* sums = reinterpret_cast<float*>(c) + ((size_t)blockIdx.y * M + row) * width + (size_t)(y / HALF) * N + n;
-        if (N % 4 == 0) {
-          store_four(sums, acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
+      for (int y = 0; y < (PARTS ? YB : HALF); ++y) {
+        const int n = ((tile_n * WN + wn) * HALF + y % HALF) * 16 + 4 * (lane / 16);
+        if (n >= N) continue;
+        if constexpr (PARTS) {
+          const size_t width = GATED ? 2 * (size_t)N : N;
+          float* sums = reinterpret_cast<float*>(c) + ((size_t)blockIdx.y * M + row) * width + (size_t)(y / HALF) * N + n;
+          if (N % 4 == 0) {
+            store_four(sums, acc[x][y][0], acc[x][y][1], acc[x][y][2], acc[x][y][3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < N) sums[e] = acc[x][y][e];
+          }
+          continue;
+        }
+        TC* at = c + (size_t)row * ldc + n;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = GATED ? f8_gate_mul(acc[x][y][e], acc[x][(y + (GATED ? HALF : 0)) % YB][e], form) : acc[x][y][e];
+        if (fours) {
+          if (accumulate) {
+            const float4 old = load_four(at);
+            v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
+          }
+          f8_store_four(at, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (n + e < N) sums[e] = acc[x][y][e];
+            if (n + e < N) at[e] = from_f32<TC>(accumulate ? v[e] + to_f32(at[e]) : v[e]);
         }
-        continue;
-      }
-      TC* at = c + (size_t)row * ldc + n;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = GATED ? f8_gate_mul(acc[x][y][e], acc[x][(y + (GATED ? HALF : 0)) % YB][e], form) : acc[x][y][e];
-      if (fours) {
-        if (accumulate) {
-          const float4 old = load_four(at);
-          v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
-        }
-        f8_store_four(at, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) at[e] = from_f32<TC>(accumulate ? v[e] + to_f32(at[e]) : v[e]);
       }
     }
   }
@@ -141,39 +191,43 @@ double cost_us(int tile, int parts, int M, int W, int K, bool full) {
 }
 
 template <typename TC, bool GATED, bool FULL, bool PARTS>
-void launch(int tile, int parts, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, int accumulate, int M, int ldc, GateForm form,
-            hipStream_t stream) {
+void launch(int tile, int parts, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, uint8_t* c_exponents, int accumulate, int M, int ldc,
+            GateForm form, hipStream_t stream) {
   const int outs = SHAPES[tile].columns / (GATED ? 2 : 1), rows = SHAPES[tile].rows;
   const dim3 grid((unsigned)(((w.rows + outs - 1) / outs) * (long)((M + rows - 1) / rows)), parts);
 #define BH_F8_RING(FULL, XB, YB, WM, WN, R, DIRECT, BM, BN)                                                                             \
-  float8_ring_kernel<TC, GATED, FULL, PARTS, XB, YB, WM, WN, R, DIRECT, BM, BN><<<grid, 64 * WM * WN, 0, stream>>>(a, exponents, w, c, M, \
-                                                                                                                  ldc, accumulate, form)
-  if (tile == 0) BH_F8_RING(FULL, 4, 4, 2, 2, 2, false, 8, 8);
-  else if (tile == 1) BH_F8_RING(FULL, 4, 4, 4, 2, 3, false, 8, 4);
-  else if (tile == 3) BH_F8_RING(FULL, 2, 4, 2, 4, 3, false, 8, 4);
+  float8_ring_kernel<TC, GATED, FULL, PARTS, XB, YB, WM, WN, R, DIRECT, BM, BN><<<grid, 64 * WM * WN, 0, stream>>>(a, exponents, w, c, \
+                                                                                                                  c_exponents, M, ldc, accumulate, form)
+  if (tile == 3) BH_F8_RING(FULL, 2, 4, 2, 4, 3, false, 8, 4);
   else if (tile == 4) BH_F8_RING(FULL, 4, 4, 2, 4, 3, false, 8, 4);
-  else if (tile == 5) BH_F8_RING(FULL, 2, 2, 2, 2, 3, false, 8, 8);
-  else if (tile == 6) BH_F8_RING(FULL, 1, 2, 2, 2, 4, false, 8, 8);
-  else if constexpr (!FULL && !PARTS) BH_F8_RING(false, 4, 8, 4, 2, 3, true, 8, 4);
+  else if (tile == 2) {
+    if constexpr (!FULL && !PARTS) BH_F8_RING(false, 4, 8, 4, 2, 3, true, 8, 4);
+  } else if constexpr (sizeof(TC) > 1) {
+    if (tile == 0) BH_F8_RING(FULL, 4, 4, 2, 2, 2, false, 8, 8);
+    else if (tile == 1) BH_F8_RING(FULL, 4, 4, 4, 2, 3, false, 8, 4);
+    else if (tile == 5) BH_F8_RING(FULL, 2, 2, 2, 2, 3, false, 8, 8);
+    else if (tile == 6) BH_F8_RING(FULL, 1, 2, 2, 2, 4, false, 8, 8);
+  }
 #undef BH_F8_RING
 }
 
 template <typename TC, bool GATED, bool FULL>
 void launch_plan(const F8RingPlan& plan, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, TC* c, float* sums, int accumulate, int M, int ldc,
                  GateForm form, hipStream_t stream) {
-  if (plan.parts == 1) launch<TC, GATED, FULL, false>(plan.tile, 1, a, exponents, w, c, accumulate, M, ldc, form, stream);
-  else launch<float, GATED, FULL, true>(plan.tile, plan.parts, a, exponents, w, sums, 0, M, ldc, form, stream);
+  if (plan.parts == 1) launch<TC, GATED, FULL, false>(plan.tile, 1, a, exponents, w, c, nullptr, accumulate, M, ldc, form, stream);
+  else launch<float, GATED, FULL, true>(plan.tile, plan.parts, a, exponents, w, sums, nullptr, 0, M, ldc, form, stream);
 }
 
 }  // namespace
 
-F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full) {
+F8RingPlan float8_ring_plan(int M, int N, int K, bool gated, bool full, bool in_stretches) {
   F8RingPlan plan = {0, 1, 0.};
   const int W = gated ? 2 * N : N, stretches = (K + F8_K - 1) / F8_K;
   for (int tile = 0; tile < TILES; ++tile) {
     if (tile == 2 && full) continue;      // (full sums have no registers for it)
+    if (in_stretches && SHAPES[tile].columns != 2 * F8_K) continue;
     const long tiles = (long)((M + SHAPES[tile].rows - 1) / SHAPES[tile].rows) * ((W + SHAPES[tile].columns - 1) / SHAPES[tile].columns);
-    const int most = tile == 2 || M > 65535 || tiles >= 2L * bh_compute_units() ? 1 : MOST_PARTS;
+    const int most = tile == 2 || in_stretches || M > 65535 || tiles >= 2L * bh_compute_units() ? 1 : MOST_PARTS;
     for (int parts = 1; parts <= most && (parts == 1 || stretches >= 4 * parts); ++parts) {
       const double cost = cost_us(tile, parts, M, W, K, full);
       if (plan.us == 0. || cost < plan.us) plan = {tile, parts, cost};
@@ -198,4 +252,12 @@ int float8_ring_launch(const F8RingPlan& plan, const uint8_t* a, const uint32_t*
 #undef BH_F8_FULL
 #undef BH_F8_RUN
   return bh_check_launch("float8_ring");
+}
+
+// The outputs of a gated product in 8 bits, a tile's being a stretch.
+int float8_ring_launch_in_8(const F8RingPlan& plan, const uint8_t* a, const uint32_t* exponents, const F8Weight& w, uint8_t* c, uint8_t* c_exponents, int through_bf16,
+                            int M, int full, GateForm form, hipStream_t stream) {
+  if (full) launch<uint8_t, true, true, false>(plan.tile, 1, a, exponents, w, c, c_exponents, through_bf16, M, w.rows, form, stream);
+  else launch<uint8_t, true, false, false>(plan.tile, 1, a, exponents, w, c, c_exponents, through_bf16, M, w.rows, form, stream);
+  return bh_check_launch("float8_ring_in_8");
 }

@@ -315,6 +315,8 @@ class KernelSizes:
             "bh_gemm_float8_few_rows": [],
             "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
+            "bh_gemm_float8_gives_8": [i, i, i, i],
+            "bh_gemm_float8_gated_to_8": [p, p, p, p, p, p, i, i, i, i, i, i, p],
             "bh_gemm_float8_rows": [p, i, p, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_route_in_groups": [p, i, p, p, p, i, i, i, i, i, i, i, i, f, p],
             "bh_experts_float8_few": [i, i],
@@ -487,6 +489,7 @@ class HipKernels(KernelSizes):
         self._squares: dict = {}    # (m, n, k) -> which product squares its output (`gemm_relu_squared`), or 0
         self._clamps: dict = {}     # (m, n, k) -> which gated product clamps (`gemm_clamped_glu`), or 0
         self._bare: dict = {}       # (m, n, k) -> the parts that `gemm_bare` leaves such a product in, or 0
+        self._float8_gives: dict = {}        # (m, n, k, full sums) -> whether a gated product leaves its outputs in 8 bits itself
         self._float8_working: dict = {}      # (rows in 8 bits already, m, n, k, gated, full sums) -> bytes that a product takes beside its output
         self._float8_experts: dict = {}      # (pairs, experts, top) -> whether they are one row's, and whether the kernels of few pairs take them
         self._float8_norm_columns = int(self.lib.bh_float8_norm_columns())
@@ -923,6 +926,28 @@ class HipKernels(KernelSizes):
         both = torch.empty((m, 2 * width), dtype=a.dtype, device=self.device)
         self.gemm(a, w, both)
         self.swiglu(both, out, gate)
+
+    def gemm_swiglu_float8(self, a, w, gate="silu", dtype=torch.float32) -> Float8Rows | None:
+        """What `gemm_swiglu` with a `Float8Weight` of two matrices would write as `dtype`, as `Float8Rows`, for a product with another that
+        alone reads it; None where the rows are few, or other kernels and `to_float8` behind them are faster (then call `gemm_swiglu`)."""
+        if not isinstance(w, Float8Weight) or w.matrices != 2 or a.dim() != 2 or a.shape[1] != w.shape[1] or dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"gemm_swiglu_float8: rows {tuple(a.shape)} and an 8-bit weight of two matrices, got {tuple(w.shape)}, to {dtype}")
+        (m, k), n, full = a.shape, w.rows, int(dtype == torch.float32)
+        key = (m, n, k, full)
+        gives = self._float8_gives.get(key)
+        if gives is None:
+            gives = self._float8_gives[key] = bool(self.lib.bh_gemm_float8_gives_8(*key))
+        if not gives:
+            return None
+        if not isinstance(a, Float8Rows):
+            a = self.to_float8(self._plain_rows(a) if type(a) is not torch.Tensor else a)
+        if a.in_rows or w.device != self.device or a.device != self.device:
+            raise KernelError(f"gemm_swiglu_float8: rows in blocks on {a.device} and a weight on {w.device}, expected {self.device}")
+        out = self._new_float8_rows(m, n, False)
+        self._check(self.lib.bh_gemm_float8_gated_to_8(
+            a.data.data_ptr(), a.exponents.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data.data_ptr(), out.exponents.data_ptr(),
+            int(dtype == torch.bfloat16), m, n, k, self.GATES[gate], full, self._stream()))
+        return out
 
     # ---- weights and rows in 8 bits ----
     def pack_float8(self, w, scales=None, matrices=1) -> Float8Weight:

@@ -50,9 +50,13 @@ class SwiGLU:
                 + self.down.working_bytes(step, step.rows, accumulate=True, then_norm=True))
 
     def forward(self, ctx, x, hidden, then_norm=None, fresh=False):
-        activated = ctx.new_activations(x.shape[0], self.intermediate, reader=self.down.reader())
-        # both products and the gate in one pass
-        ctx.kernels.gemm_swiglu(x, self.gate_up.weight, activated, **({} if self.GATE == "silu" else {"gate": self.GATE}))
+        gate = {} if self.GATE == "silu" else {"gate": self.GATE}
+        in_float8 = getattr(ctx.kernels, "gemm_swiglu_float8", None) if self.gate_up.float8 and self.down.float8 else None
+        activated = in_float8(x, self.gate_up.weight, dtype=ctx.act_dtype, **gate) if in_float8 is not None else None
+        if activated is None:
+            activated = ctx.new_activations(x.shape[0], self.intermediate, reader=self.down.reader())
+            # both products and the gate in one pass
+            ctx.kernels.gemm_swiglu(x, self.gate_up.weight, activated, **gate)
         if fresh:
             self.down.forward(ctx, activated, out=hidden)
             return None

@@ -54,3 +54,27 @@ def test_experts_refuse(sizes):
 def test_sizes():
     assert Float8Weight.data_bytes(2, 17, 129) == 2 * 32 * 256 and Float8Weight.scale_shape(2, 129, 129) == (2, 2, 2)
     assert Float8Rows.bytes_of(17, 513) == (32 * 640, 4 * 32 * 2)
+
+
+def test_products_between_rows_in_8_bits_refuse(sizes):
+    lib = sizes.lib
+    assert lib.bh_gemm_float8_rows(AT, 0, None, AT, AT, AT, 0, 0, 40, 16, 128, 16, 0, 1, None) != 0
+    assert lib.bh_gemm_float8_rows(AT, 7, AT, AT, AT, AT, 0, 0, 40, 16, 128, 16, 0, 1, None) != 0
+    assert lib.bh_gemm_float8_rows(AT, 0, AT, AT + 8, AT, AT, 0, 0, 40, 16, 128, 16, 0, 1, None) != 0
+    for m, n, k, gate, at in ((127, 256, 128, 1, AT), (400, 0, 128, 1, AT), (400, 256, 0, 1, AT), (400, 256, 128, 0, AT), (400, 256, 128, 9, AT), (400, 256, 128, 1, AT + 8)):
+        assert lib.bh_gemm_float8_gated_to_8(AT, AT, at, AT, AT, AT, 0, m, n, k, gate, 1, None) != 0
+        assert b"gemm_float8" in lib.bh_last_error()
+    for rows, width, dtype, at in ((0, 128, 0, AT), (1, 0, 0, AT), (1, 8193, 0, AT), (1, 128, 5, AT), (1, 128, 0, AT + 4)):
+        assert lib.bh_float8_norm(AT, AT, dtype, 1e-5, 0, at, AT, rows, width, None) != 0
+        assert b"float8_norm" in lib.bh_last_error()
+
+
+@pytest.mark.parametrize("n,k,gated", [(1024, 4096, False), (4096, 12288, False), (300, 5000, True)])
+def test_the_plan_of_many_rows_counts_what_fewer_rows_take(sizes, n, k, gated):
+    """K is cut into parts where the rows are few: a step of fewer rows than the plan's largest may need more for their sums."""
+    planned = sizes.gemm_float8_working_bytes(1000, n, k, 2, gated)
+    rows = sum(Float8Rows.bytes_of(1000, k))
+    for m in range(17, 1001):
+        for full in (0, 1):
+            assert planned >= rows + sizes.lib.bh_gemm_float8_scratch(m, n, k, int(gated), full)
+    assert max(sizes.lib.bh_gemm_float8_scratch(m, n, k, int(gated), 1) for m in range(17, 1000)) > sizes.lib.bh_gemm_float8_scratch(1000, n, k, int(gated), 1)

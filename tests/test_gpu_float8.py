@@ -407,6 +407,42 @@ def test_every_kernel_of_products_from_rows_in_8_bits(k, m, n, width, full, gate
     assert bool(torch.isfinite(out).all())
 
 
+@pytest.mark.parametrize("m,n,width", [(400, 4100, 130), (130, 700, 300), (700, 12288, 512), (2100, 6000, 384), (1000, 4100, 1000), (5000, 300, 130)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", ["silu", "gelu_tanh"])
+def test_gated_products_that_leave_rows_in_8_bits(k, m, n, width, dtype, gate):
+    """The bytes of `gemm_swiglu` and `to_float8` behind it where both add up in the same order, which within a step they do; else what lies at a
+    border falls on its other side.  And rows in 8 bits are read by the next product."""
+    x, (w, _) = _rows(m, width, torch.bfloat16, 3).to(DEVICE), _weight(k, 2, n, width, 4)
+    got = k.gemm_swiglu_float8(x, w, gate=gate, dtype=dtype)
+    plainly = torch.empty((m, n), dtype=dtype, device=DEVICE)
+    k.gemm_swiglu(x, w, plainly, gate=gate)
+    want = k.to_float8(plainly)
+    assert (got is not None) == bool(k.lib.bh_gemm_float8_gives_8(m, n, width, int(dtype == torch.float32)))
+    if got is None:
+        return
+    a, b = k.from_float8(got), k.from_float8(want)
+    assert bool(torch.isfinite(a).all()) and (a != b).double().mean().item() < 0.01
+    # a step of e4m3 is 2^-3 of a value at most, and values below the smallest normal number of their stretch lie 2^-9 * 2^e apart
+    least = torch.ldexp(torch.ones((), device=DEVICE), torch.frexp(plainly.float().abs().amax(dim=1, keepdim=True))[1] - 8 - 9 + 1)
+    assert bool(((a - b).abs() <= torch.maximum(b.abs() * 0.1251, least)).all())
+    v, _ = _weight(k, 1, 64, n, 5)
+    first, second = torch.empty((m, 64), device=DEVICE), torch.empty((m, 64), device=DEVICE)
+    k.gemm(got, v, first)
+    k.gemm(want, v, second)
+    assert float((first - second).norm() / second.norm()) < 0.0126      # 1 % of the values a step of 2^-3 off
+
+
+def test_gated_products_that_do_not_leave_rows_in_8_bits(k):
+    from beholdd.kernels.library import KernelError
+    w = _weight(k, 2, 64, 128, 4)[0]
+    assert k.gemm_swiglu_float8(torch.ones((4, 128), device=DEVICE), w) is None
+    for call in (lambda: k.gemm_swiglu_float8(torch.ones((400, 64), device=DEVICE), w), lambda: k.gemm_swiglu_float8(torch.ones((400, 128), device=DEVICE), _weight(k, 1, 64, 128, 4)[0]),
+                 lambda: k.gemm_swiglu_float8(torch.ones((400, 128), device=DEVICE), w, dtype=torch.float16)):
+        with pytest.raises(KernelError):
+            call()
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 def test_refusals(k):
