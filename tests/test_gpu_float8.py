@@ -384,6 +384,17 @@ def test_tiles_and_parts_of_k(k, m, n, width, full):
     assert bool(torch.isfinite(out).all())
 
 
+@pytest.mark.parametrize("m", [3, 20, 70, 300])
+def test_several_matrices_side_by_side(k, m):
+    """A plain product with a weight of three matrices: their outputs behind one another in each row, added to what is there."""
+    x, (w, held) = _rows(m, 300, torch.bfloat16, 1), _weight(k, 3, 50, 300, 2)
+    before = torch.randn((m, 150), generator=torch.Generator().manual_seed(3))
+    out = before.to(DEVICE)
+    k.gemm(x.to(DEVICE), w, out, accumulate=True)
+    want, bound = plain.product(plain.rows(x), plain.matrix(*held), True)
+    _close(out, want + before.double(), bound + (want.abs() + before.abs().double()) * 2.0 ** -24)
+
+
 @pytest.mark.parametrize("m,n,width,full,gated", [
     (20, 130, 640, False, False), (20, 130, 640, True, True), (48, 130, 384, True, False), (60, 130, 384, False, False), (60, 100, 384, True, True),
     (90, 130, 384, False, False), (90, 130, 384, True, True), (128, 130, 384, True, False), (100, 2050, 640, False, False), (100, 130, 3000, False, False),
