@@ -54,6 +54,25 @@ def test_every_cut_of_the_work(folder, dtype):
     assert _off(batch, want[[6, 39, 89]]) < 2 * NORM[dtype]      # (three rows rather than 150: their norm varies more)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("batch", [20, 60, 130])
+def test_captured_steps_of_many_sequences(folder, dtype, batch):
+    """Every replay of a step whose norms write rows in 8 bits, with eager steps between, as the CPU's engine has the same positions."""
+    engine = beholdd.Engine(folder, dtype=dtype, max_tokens=(batch + 1) * 64, max_slots=batch + 1, device="cuda:0", weights="float8")
+    double = beholdd.Engine(folder, dtype=dtype, max_tokens=512, device="cpu", kernels=Float8TorchKernels(), weights="float8")
+    prompt = [int(t) for t in np.random.default_rng(8).integers(0, 384, size=40)]
+    want = double.step([beholdd.StepEntry(double.alloc_slot(), prompt, list(range(40)))])
+    slots, lengths = [engine.alloc_slot() for _ in range(batch)], [5 + i % 25 for i in range(batch)]
+    engine.step([beholdd.StepEntry(slot, prompt[:n], [n - 1]) for slot, n in zip(slots, lengths)])
+    for t in range(6):
+        got = engine.step([beholdd.StepEntry(slot, [prompt[n + t]], [0]) for slot, n in zip(slots, lengths)]).clone()
+        assert _off(got, want[[n + t for n in lengths]]) < 2 * NORM[dtype], f"step {t}"
+        other = engine.alloc_slot()
+        engine.step([beholdd.StepEntry(other, prompt[:30], [29])])
+        engine.free_slot(other)
+        torch.cuda.synchronize()
+
+
 def test_generation_in_8_bits(folder):
     """Greedy tokens of the loop that runs ahead are those of its own steps one by one."""
     engine = beholdd.Engine(folder, dtype="bfloat16", max_tokens=1024, device="cuda:0", weights="float8")
