@@ -4,10 +4,10 @@
 //   float8_norm   the RMSNorm of float32 rows, x / sqrt(mean(x^2) + eps) * w, of float32 or of the bfloat16 that it is elsewhere
 //
 // 16 lanes hold a stretch of 128 values, 8 each (16 bytes of bfloat16), a wave four stretches of a row: its largest magnitude takes four
-// steps between neighbouring lanes, the exponents of the four stretches make one word.  A workgroup of four waves takes the 16 rows of a
-// block, four a wave that are loaded together, so that the 256-byte runs of a block that its rows write in pieces of 8 bytes meet in one L2;
-// of few rows a wave takes one, which is the shorter chain.
-// Measured, us: 2,048 x 4,096 bfloat16 7.7, 8,160 x 4,096 28.3 (3.6 TB/s; 35.4 with the rows one after the other), 45 x 12,288 2.6 (5.0).
+// steps between neighbouring lanes, the exponents of the four stretches make one word.  A block's runs of 256 bytes are written by its 16 rows in pieces of 8
+// bytes: from 4,096 pieces of 512 columns on a workgroup takes a row, and the 16 rows of a block run on one XCD, so that the pieces meet in one L2.
+// Measured, us, in brackets with four rows a wave in workgroups of a block: 512 x 4,096 bfloat16 3.1 (4.0), 2,048 x 4,096 6.5 (7.2), 8,160 x 4,096 22.4 (26.7, 4.5 TB/s), 8,192 x
+// 12,288 64.6 (80); few rows that way 2.7, in pieces of four rows 2.3 (45 x 12,288).
 #include "float8.h"
 
 namespace {
@@ -36,7 +36,7 @@ __device__ inline uint32_t turned(uint32_t v) {
 }
 
 // A lane's eight values of a row from column k on, in 8 bits; 64 lanes hold 512 neighbouring columns, a word of exponents.
-__device__ inline void eight_in_8(const float (&v)[8], long row, bool exists, int k, int stretches, int padded, int in_rows, uint8_t* __restrict__ data,
+__device__ inline void eight_in_8(const float (&v)[8], long row, int k, int stretches, int padded, int in_rows, uint8_t* __restrict__ data,
                                   uint32_t* __restrict__ exponents) {
   const int lane = threadIdx.x % 64, stretch = k / F8_K;
   uint32_t largest = 0;
@@ -48,55 +48,49 @@ __device__ inline void eight_in_8(const float (&v)[8], long row, bool exists, in
   largest = max(largest, turned<1>(largest));
   const uint32_t exponent = f8_exponent(largest);
   const float scale = f8_scale(exponent);
-  if (exists && stretch < stretches) {
+  if (stretch < stretches) {
     const uint2 eight = make_uint2(f8_four(v[0], v[1], v[2], v[3], scale), f8_four(v[4], v[5], v[6], v[7], scale));
     const long at = in_rows ? (row * stretches + stretch) * F8_K + k % F8_K
                             : (row / 16 * stretches + stretch) * F8_BLOCK + f8_place((int)(row % 16), k % F8_K);
     *reinterpret_cast<uint2*>(data + at) = eight;
   }
   const uint32_t word = f8_over_rows(exponent << (8 * (lane / 16)), [](uint32_t a, uint32_t b) { return a | b; });
-  if (lane == 0 && exists) exponents[(long)(k / 512) * padded + row] = word;
+  if (lane == 0) exponents[(long)(k / 512) * padded + row] = word;
 }
 
-// grid (ceil(rows / (4 EACH)), ceil(width / 512)).  EACH: rows of a wave.
+// SPREAD false: grid (ceil(rows / 4), ceil(width / 512)), 512 columns of four rows a workgroup.  True: grid (whole rounds of rows, ceil(width / 4,096)), up to
+// 4,096 columns of a row a workgroup, the 16 rows of a block on one XCD.
 // `in_rows`: row after row instead, each of whole stretches (what the experts' products pick their rows from).
-template <typename T, bool GATED, bool WHOLE, int EACH>
-__global__ __launch_bounds__(256) void float8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ data, uint32_t* __restrict__ exponents,
+template <typename T, bool GATED, bool WHOLE, bool SPREAD>
+__global__ __launch_bounds__(512) void float8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ data, uint32_t* __restrict__ exponents,
                                                           int rows, int width, int in_rows, GateForm form) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int stretches = (width + F8_K - 1) / F8_K, k = blockIdx.y * 512 + lane * 8;
-  const int padded = (rows + 15) / 16 * 16;
-  const long first = ((long)blockIdx.x * 4 + wave) * EACH;
-  float v[EACH][8];
+  const int stretches = (width + F8_K - 1) / F8_K, padded = (rows + 15) / 16 * 16;
+  const int row = SPREAD ? bh_row_of_block<true>() : (int)(blockIdx.x * 4 + threadIdx.x / 64);
+  const int k = SPREAD ? (int)(blockIdx.y * blockDim.x + threadIdx.x) * 8 : (int)(blockIdx.y * 512 + threadIdx.x % 64 * 8);
+  if (row >= rows || k / 512 * 512 >= width) return;      // the whole wave
+  const T* from = x + (size_t)row * (GATED ? 2L * width : (long)width);
+  float v[8];
+  load_eight<T, WHOLE>(from, k, width, v);
+  if constexpr (GATED) {
+    float u[8];
+    load_eight<T, WHOLE>(from + width, k, width, u);
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const T* from = x + min(first + i, (long)rows - 1) * (GATED ? 2L * width : (long)width);
-    load_eight<T, WHOLE>(from, k, width, v[i]);
-    if constexpr (GATED) {
-      float u[8];
-      load_eight<T, WHOLE>(from + width, k, width, u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = f8_gate_mul(v[i][j], u[j], form);
-    }
+    for (int j = 0; j < 8; ++j) v[j] = f8_gate_mul(v[j], u[j], form);
   }
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const long row = first + i;
-    eight_in_8(v[i], row, row < rows, k, stretches, padded, in_rows, data, exponents);
-  }
+  eight_in_8(v, row, k, stretches, padded, in_rows, data, exponents);
 }
 
 template <typename T>
 void launch(const void* x, uint8_t* data, uint32_t* exponents, int rows, int width, int in_rows, int gate, hipStream_t stream) {
   const bool whole = width % 8 == 0 && (uintptr_t)x % 16 == 0;
-  const bool few = (long)rows * ((width + 511) / 512) < 16L * bh_compute_units();      // waves' worth of work: four a wave would leave SIMDs without
-  const dim3 grid((rows + (few ? 3 : 15)) / (few ? 4 : 16), (width + 511) / 512);
+  const int pieces = (width + 511) / 512, waves = pieces < 8 ? pieces : 8;
+  const bool few = (long)rows * pieces < 16L * bh_compute_units();
   const GateForm form = bh_gate_form(gate);
-#define BH_F8_ROWS_OF(GATED, WHOLE, EACH) float8_rows_kernel<T, GATED, WHOLE, EACH><<<grid, 256, 0, stream>>>((const T*)x, data, exponents, rows, width, in_rows, form)
-#define BH_F8_ROWS(GATED, WHOLE)                 \
-  do {                                           \
-    if (few) BH_F8_ROWS_OF(GATED, WHOLE, 1);     \
-    else BH_F8_ROWS_OF(GATED, WHOLE, 4);         \
+  const dim3 grid = few ? dim3((rows + 3) / 4, pieces) : dim3(((unsigned)rows + BH_ROWS_ROUND - 1) / BH_ROWS_ROUND * BH_ROWS_ROUND, (pieces + waves - 1) / waves);
+#define BH_F8_ROWS(GATED, WHOLE)                                                                                                                              \
+  do {                                                                                                                                                        \
+    if (few) float8_rows_kernel<T, GATED, WHOLE, false><<<grid, 256, 0, stream>>>((const T*)x, data, exponents, rows, width, in_rows, form);                   \
+    else float8_rows_kernel<T, GATED, WHOLE, true><<<grid, waves * 64, 0, stream>>>((const T*)x, data, exponents, rows, width, in_rows, form);                 \
   } while (0)
   if (gate) {
     if (whole) BH_F8_ROWS(true, true);
@@ -104,7 +98,6 @@ void launch(const void* x, uint8_t* data, uint32_t* exponents, int rows, int wid
   } else if (whole) BH_F8_ROWS(false, true);
   else BH_F8_ROWS(false, false);
 #undef BH_F8_ROWS
-#undef BH_F8_ROWS_OF
 }
 
 // A row is a workgroup's, 512 columns a wave's, read once.  The 16 rows of a block, whose pieces of 8 bytes share lines, are the work of one XCD.
@@ -138,7 +131,7 @@ __global__ __launch_bounds__(1024) void float8_norm_kernel(const float* __restri
     v[j] = k + j < width ? v[j] * inv * g[j] : 0.f;
     if (through_bf16) v[j] = to_f32(from_f32<bf16_t>(v[j]));
   }
-  eight_in_8(v, row, true, k, stretches, padded, 0, data, exponents);
+  eight_in_8(v, row, k, stretches, padded, 0, data, exponents);
 }
 
 template <typename TW>
