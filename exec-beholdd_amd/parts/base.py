@@ -36,6 +36,8 @@ A matrix that one product alone reads may be kept the way that product reads it 
     consumer with `input_reader` (a ProductReader: the product its `x` goes to, and nowhere else): its `x` may
         then be in the kernel library's own form for that product; it hands `x` to that product untouched.
     norm with `serves_reader = True`: forward(..., reader=) and request(reader) take that ProductReader.
+    A reader that says `float8` may get rows in 8 bits, which no other operation reads or regroups: a block whose norm
+    has several readers says so only where all of them do.
     Inside a part, `ctx.new_activations(rows, width, reader=linear.reader())` asks for such a matrix between two
     of its own kernel calls.  Parts that say nothing get and give plain matrices.
 A mixer with a "state" cache need moves its rows of `cache.state` on while it runs: in place, at the rows `ctx.seq_slot`

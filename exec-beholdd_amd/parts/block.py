@@ -7,6 +7,8 @@ and is updated in place; the mixer and the feed-forward add into it.  `SharedNor
 
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
 from .base import BLOCKS, FEED_FORWARDS, MIXERS, NORMS, graph_rows_allowed
@@ -197,9 +199,15 @@ class SharedNormBlock:
 
     def _reader(self):
         """The product in whose form the norm's output is kept: the feed-forward's or else the mixer's (whoever reads it in another
-        form regroups it)."""
+        form regroups it).  Rows in 8 bits are no form that another reader could regroup: they are for sublayers that both hand them to
+        a product which takes them."""
+        if not getattr(self.norm, "serves_reader", False):
+            return None
         part = self.feed_forward if self.feed_forward is not None else self.mixer
-        return getattr(part, "input_reader", None) if getattr(self.norm, "serves_reader", False) else None
+        reader = getattr(part, "input_reader", None)
+        if getattr(reader, "float8", False) and not getattr(getattr(self.mixer, "input_reader", None), "float8", False):
+            reader = replace(reader, float8=False)
+        return reader
 
     def forward(self, ctx, hidden, cache, prepared=None, next_block=None):
         """`hidden` [rows, width] float32, updated in place.  `prepared`: this block's norm of it, if the block before made it; returns
