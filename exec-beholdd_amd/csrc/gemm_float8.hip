@@ -157,6 +157,12 @@ int span_of(int N, int K, bool gated) {
   return 16;
 }
 
+// The span that `few` runs with.  Plain bfloat16 rows and rows in 8 bits have other spans than 16 (float32 rows go in whole blocks: they are not what
+// a step of few rows has as a rule).
+int few_span(int N, int K, bool gated, size_t row_element, int load) {
+  return row_element <= 2 && load == F8_EVEN ? span_of(N, K, gated) : 16;
+}
+
 // Blocks of 16 rows that the kernel for M rows is compiled for.
 int few_row_blocks(int M) { return M <= 32 ? 2 : M <= 48 ? 3 : M <= 64 ? 4 : M <= 96 ? 6 : 8; }
 
@@ -184,8 +190,8 @@ bool few_takes(int M, int N, int K, bool gated, bool full, F8RingPlan* plan) {
 template <typename T, typename TC, bool GATED, bool FULL, int MB>
 void launch_few_blocks(const void* x, const uint32_t* exponents, const F8Weight& w, TC* c, int M, int K, int ldc, int accumulate, GateForm form, hipStream_t stream) {
   const int load = sizeof(T) == 1 ? (int)F8_EVEN : f8_load_of(x, K);
-  constexpr bool SPANS = sizeof(T) <= 2 && !GATED;      // (float32 rows go in whole blocks: they are not what a step of few rows has as a rule)
-  const int span = SPANS && load == F8_EVEN ? span_of(w.rows, K, GATED) : 16;
+  constexpr bool SPANS = sizeof(T) <= 2 && !GATED;
+  const int span = few_span(w.rows, K, GATED, sizeof(T), load);
   const dim3 grid((w.rows + span - 1) / span);
 #define BH_F8_FEW(NB, LOAD, MASKED, DEPTH)                                                                                            \
   few_kernel<T, TC, MB, NB, GATED, FULL, LOAD, MASKED, DEPTH><<<grid, FEW_WAVES * 64, 0, stream>>>((const T*)x, exponents, w, c, M, K, \
@@ -243,6 +249,19 @@ extern "C" long bh_gemm_float8_scratch(int M, int N, int K, int gated, int full)
   F8RingPlan plan;
   if (M <= 0 || N <= 0 || K <= 0 || few_takes(M, N, K, gated != 0, full != 0, &plan)) return 0;
   return plan.parts > 1 ? (long)plan.parts * M * N * (gated ? 2 : 1) * 4 : 0;
+}
+
+// Which kernel a product runs on, from rows of `dtype` on addresses of 16 bytes or (dtype -1) in 8 bits: kernel[0] blocks of 16 rows that `few` is
+// compiled for and kernel[1] its span, or 0 and 0; kernel[2] the rings' tile and kernel[3] its parts, or -1 and 0.
+extern "C" int bh_gemm_float8_kernel(int dtype, int M, int N, int K, int gated, int full, int* kernel) {
+  BH_REQUIRE(M > 0 && N > 0 && K > 0 && kernel != nullptr, "gemm_float8: sizes must be positive, got %d x %d x %d", M, N, K);
+  F8RingPlan plan = {-1, 0, 0.};
+  const bool plain = dtype >= 0 && M <= FEW_ROWS, few = plain || few_takes(M, N, K, gated != 0, full != 0, &plan);
+  kernel[0] = plain ? 1 : few ? few_row_blocks(M) : 0;
+  kernel[1] = !few ? 0 : few_span(N, K, gated != 0, plain ? (dtype == BH_F32 ? 4 : 2) : 1, plain ? f8_load_of(nullptr, K) : F8_EVEN);
+  kernel[2] = few ? -1 : plan.tile;
+  kernel[3] = few ? 0 : plan.parts;
+  return 0;
 }
 
 #define BH_F8_BY_TYPES(RUN)                                                                                        \

@@ -313,6 +313,7 @@ class KernelSizes:
             "bh_float8_norm_columns": [],
             "bh_float8_norm": [p, p, i, f, i, p, p, i, i, p],
             "bh_gemm_float8_few_rows": [],
+            "bh_gemm_float8_kernel": [i, i, i, i, i, i, p],
             "bh_gemm_float8_few": [p, i, p, p, p, i, i, i, i, i, i, i, i, p],
             "bh_gemm_float8": [p, p, p, p, p, i, i, i, i, i, i, i, i, p, p],
             "bh_gemm_float8_gives_8": [i, i, i, i],
