@@ -118,13 +118,20 @@ __device__ inline f8_f32x4_t f8_stretch(const F8Operand<true>& w, const F8Operan
   return sum;
 }
 
-// g / (1 + exp(-y)) by the instructions for 2^x and 1 / x, each within a unit in the last place of float32; the exponent's rounding leaves 2^-24 |y| of
-// the exponential, which is small beside 1 where y is large and makes a share of 2^-24 |y| of a value that is itself as small as exp(-|y|) where it
-// is not.  A tile's end has 64 of these a lane: with the library's exponential and division they were 12 % of a gated product's time.
+// g / (1 + exp(-y)) by the instructions for 2^x and 1 / x, each within a unit in the last place of float32, for values that are rounded to bfloat16 or to
+// 8 bits next: the exponent's rounding leaves 2^-24 |y| of the exponential (7e-6 of a value at y = -80, where a step of bfloat16 is 8e-3), and where
+// exp(-y) exceeds 2^126 (a value of 1e-36 and less) 1 / x may be flushed to zero.  A tile's end has 64 of these a lane: with the library's
+// exponential and division they were 12 % of a gated product's time.
 __device__ inline float f8_gated(float g, float y) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * y));
 }
 __device__ inline float f8_gate_mul(float g, float u, GateForm form) { return f8_gated(g, g * fmaf(form.cube, g * g, form.slope)) * u; }
+// A gated output of type TC: a float32 one by the library's exponential and division, within float32's errors of the activation wherever it lies.
+template <typename TC>
+__device__ inline float f8_gate_out(float g, float u, GateForm form) {
+  if constexpr (sizeof(TC) == 4) return gate_mul(g, u, form);
+  else return f8_gate_mul(g, u, form);
+}
 
 // A weight of `matrices` matrices [rows][K] as the kernels see it.
 struct F8Weight {

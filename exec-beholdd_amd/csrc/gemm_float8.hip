@@ -119,7 +119,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(const T* __restrict
         for (int v = 0; v < FEW_WAVES; ++v) sum[g] += partial[v][g * NB + t][b][e % 256];
       }
       TC* at = c + (size_t)m * ldc + n;
-      float value = GATED ? f8_gate_mul(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
+      float value = GATED ? f8_gate_out<TC>(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
       if (accumulate) value += to_f32(*at);
       *at = from_f32<TC>(value);
     }
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ s
     for (int p = 0; p < parts; ++p) sum[g] += sums[((size_t)p * M + row) * width + g * N + n];
   }
   TC* at = c + (size_t)row * ldc + n;
-  float value = GATED ? f8_gate_mul(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
+  float value = GATED ? f8_gate_out<TC>(sum[0], sum[GATED ? 1 : 0], form) : sum[0];
   if (accumulate) value += to_f32(*at);
   *at = from_f32<TC>(value);
 }

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void float8_ring_kernel(const uint
         TC* at = c + (size_t)row * ldc + n;
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = GATED ? f8_gate_mul(acc[x][y][e], acc[x][(y + (GATED ? HALF : 0)) % YB][e], form) : acc[x][y][e];
+        for (int e = 0; e < 4; ++e) v[e] = GATED ? f8_gate_out<TC>(acc[x][y][e], acc[x][(y + (GATED ? HALF : 0)) % YB][e], form) : acc[x][y][e];
         if (fours) {
           if (accumulate) {
             const float4 old = load_four(at);
