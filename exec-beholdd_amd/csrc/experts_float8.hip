@@ -2,6 +2,7 @@
 //   inner[p] = act(Wg_e x[row], Wu_e x[row])     act(g, u) = g' / (1 + exp(-alpha g')) * (u' + shift), g' = min(g, limit), u' = clamp(u, +-limit)
 //   y[p]     = Wd_e inner[p]                     inner in 32 bits, brought into 8 once
 //   out[row] (+)= sum over j of weight[p] * y[p], j in order
+// A sum that is not a number stays one behind a finite limit, as it does without: its inner value becomes e4m3's NaN, and its row's outputs NaN.
 // A pair's weight may multiply the expert's input instead (its gate and up sums).  A pair whose expert is none of the E gives nothing, or,
 // with `through`, one numbered E or higher hands the row's input on.  Nothing here depends on the routing on the host.
 //   one    the pairs of one row
@@ -16,8 +17,8 @@ struct ExpertGate {
   float limit, alpha, shift;
 };
 __device__ inline float activated(float g, float u, const ExpertGate& gate) {
-  g = fminf(g, gate.limit);
-  u = fminf(fmaxf(u, -gate.limit), gate.limit);
+  g = g > gate.limit ? gate.limit : g;      // (fminf and fmaxf would give the limit for a NaN)
+  u = u > gate.limit ? gate.limit : u < -gate.limit ? -gate.limit : u;
   return f8_gated(g, gate.alpha * g) * (u + gate.shift);
 }
 
