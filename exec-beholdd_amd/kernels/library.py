@@ -323,7 +323,7 @@ class KernelSizes:
             "bh_experts_float8_few": [i, i],
             "bh_experts_float8_rows": [p, i, i, p, i, i, p, p, p, i, i, i, f, f, f, p, i, p],
             "bh_experts_float8_one": [i, i],
-            "bh_experts_float8_row": [p, i, p, p, i, p, i, p, p, p, p, p, p, i, i, i, i, i, f, f, f, i, i, i, p],
+            "bh_experts_float8_row": [p, i, p, p, i, p, i, p, p, p, p, p, p, i, i, i, i, i, f, f, f, i, i, p],
             "bh_experts_float8_tiles": [p, p, i, i, p, i, p, i, i, p, p, p, p, i, i, i, f, f, f, p, i, p],
             "bh_experts_float8_sum": [p, p, p, p, i, p, i, i, i, i, i, i, p],
         }
@@ -1108,9 +1108,9 @@ class HipKernels(KernelSizes):
         chosen int32 [n, top], weights float32 [n, top]; `w_up` a `Float8Weight` of 2 E matrices [ff, K] (gate and up of each expert in turn),
         `w_down` one of E matrices [D, ff], out [n, D] float32 or bfloat16.  `weigh_input`: a pair's weight multiplies the expert's input in
         place of its output.  A pair whose expert is none of the E counts nothing; with `through` [n, D] (of x's type) one that is numbered
-        E or higher gives through[r].  x and the activations go into the products in 8 bits (`to_float8`); `full_sums` as in `gemm`, but if it
-        is not said the gate and up sums are full: they are rounded to 8 bits, and each that falls on the other side of a border is a whole
-        step off (4,096 rows of 4,096, bfloat16 output: 2.6e-3 of it, 1.7e-3 with full sums, where its own rounding is 1.6e-3)."""
+        E or higher gives through[r].  x and the activations go into the products in 8 bits (`to_float8`).  `full_sums` says how the last product
+        adds up, as in `gemm`.  The gate and up sums are always full: they are rounded to 8 bits, and each that falls on the other side of a
+        border is a whole step off."""
         if not isinstance(w_up, Float8Weight) or not isinstance(w_down, Float8Weight) or x.dim() != 2 or chosen.dim() != 2:
             raise KernelError("experts_float8: rows, choices [n, top] and two 8-bit weights")
         (n, k), top, experts, ff, width = x.shape, chosen.shape[1], w_down.matrices, w_up.rows, w_down.rows
@@ -1123,7 +1123,7 @@ class HipKernels(KernelSizes):
             raise KernelError(f"experts_float8: weights on {w_up.device} and {w_down.device}, expected {self.device}")
         if through is not None and weigh_input:
             raise KernelError("experts_float8: inputs that are handed through are weighed on their way out")
-        full, full_up = out.dtype == torch.float32 if full_sums is None else bool(full_sums), full_sums is None or bool(full_sums)
+        full = out.dtype == torch.float32 if full_sums is None else bool(full_sums)
         lib, stream, pairs = self.lib, self._stream(), n * top
         chosen_at, weights_at = self._ptr(chosen, "chosen", (torch.int32,)), self._ptr(weights, "route weights", (torch.float32,), True)
         act = (float(limit), float(alpha), float(shift))
@@ -1137,14 +1137,14 @@ class HipKernels(KernelSizes):
             inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
             self._check(lib.bh_experts_float8_row(
                 x_at, x_code, chosen_at, weights_at, int(weigh_input), through_at, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), w_down.data.data_ptr(),
-                w_down.scales.data_ptr(), inner.data_ptr(), out_at, out_code, top, k, ff, width, *act, int(bool(fresh)), int(full_up), int(full), stream))
+                w_down.scales.data_ptr(), inner.data_ptr(), out_at, out_code, top, k, ff, width, *act, int(bool(fresh)), int(full), stream))
             return
         in_weights, out_weights = (weights_at, None) if weigh_input else (None, weights_at)
         y = torch.empty((pairs, width), dtype=torch.float32, device=self.device)
         if few:
             inner = torch.empty((pairs, ff), dtype=torch.float32, device=self.device)
             self._check(lib.bh_experts_float8_rows(x_at, x_code, top, chosen_at, pairs, experts, w_up.data.data_ptr(), w_up.scales.data_ptr(), inner.data_ptr(),
-                                                   ff, k, 1, *act, in_weights, int(full_up), stream))
+                                                   ff, k, 1, *act, in_weights, 1, stream))
             self._check(lib.bh_experts_float8_rows(inner.data_ptr(), F32, 1, chosen_at, pairs, experts, w_down.data.data_ptr(), w_down.scales.data_ptr(),
                                                    y.data_ptr(), width, ff, 0, *act, None, int(full), stream))
         else:
@@ -1153,7 +1153,7 @@ class HipKernels(KernelSizes):
             self._check(lib.bh_experts_group(chosen_at, pairs, lists.data_ptr(), pairs, counts.data_ptr(), experts, stream))
             rows, inner = self.to_float8(x, in_rows=True), self._new_float8_rows(pairs, ff, True)
             for a, in_rows, div, w, out_rows, out_exponents, outs, ins, is_full in (
-                    (rows, n, top, w_up, inner.data, inner.exponents, ff, k, full_up), (inner, pairs, 1, w_down, y, None, width, ff, full)):
+                    (rows, n, top, w_up, inner.data, inner.exponents, ff, k, True), (inner, pairs, 1, w_down, y, None, width, ff, full)):
                 gated = out_exponents is not None
                 self._check(lib.bh_experts_float8_tiles(
                     a.data.data_ptr(), a.exponents.data_ptr(), in_rows, div, lists.data_ptr(), pairs, counts.data_ptr(), pairs, experts, w.data.data_ptr(),

@@ -48,3 +48,12 @@ def test_refusals(lib):
     kernel = (ctypes.c_int * 4)()
     for m, n, k, to in ((0, 16, 128, kernel), (1, 0, 128, kernel), (1, 16, 0, kernel), (1, 16, 128, None)):
         assert lib.bh_gemm_float8_kernel(-1, m, n, k, 0, 0, to) != 0
+
+
+def test_gate_and_up_sums_of_experts_are_full(lib):
+    """The C entries refuse to make them otherwise, before anything is launched."""
+    at = 4096
+    assert lib.bh_experts_float8_rows(at, 0, 1, at, 4, 4, at, at, at, 16, 128, 1, 1.0, 1.0, 0.0, None, 0, None) != 0
+    assert b"in full" in lib.bh_last_error()
+    assert lib.bh_experts_float8_tiles(at, at, 4, 1, at, 4, at, 4, 4, at, at, at, at, 16, 128, 1, 1.0, 1.0, 0.0, None, 0, None) != 0
+    assert b"in full" in lib.bh_last_error()
