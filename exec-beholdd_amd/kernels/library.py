@@ -390,6 +390,18 @@ class KernelSizes:
             total += sum(_rounded(size) for size in Float8Rows.bytes_of(m, k)) + _rounded(scratch)
         return total
 
+    def experts_float8_working_bytes(self, n, top, experts, width, ff) -> int:
+        """The most bytes that `experts_float8` allocates for up to `n` rows: the pairs' results, and either their inner values in float32 (few
+        pairs) or the experts' lists, the rows and the inner values in 8 bits (which have whole stretches, and exponents)."""
+        pairs, experts = int(n) * int(top), int(experts)
+        few, above = 0, pairs + 1      # the largest number of pairs that counts as few
+        while above - few > 1:
+            middle = (few + above) // 2
+            few, above = (middle, above) if self.lib.bh_experts_float8_few(middle, experts) else (few, middle)
+        total = 0 if few == pairs else (_rounded(4 * experts * pairs) + _rounded(4 * experts)
+                                        + sum(_rounded(size) for shape in ((n, width), (pairs, ff)) for size in Float8Rows.bytes_of(*map(int, shape))))
+        return _rounded(4 * pairs * int(width)) + max(total, _rounded(4 * max(few, int(top)) * int(ff)))
+
     def float8_bytes(self, matrices, rows, cols) -> int:
         """Device bytes of `matrices` matrices [rows, cols] as `pack_float8` keeps them."""
         count = 1

@@ -201,8 +201,9 @@ class RoutedExperts:
             total = step.matrix(step.rows, self.WIDE_ROUTER, 4) + step.product(step.rows, self.WIDE_ROUTER, self.hidden)
         total += 2 * step.matrix(step.rows, self.top, 4)
         pairs = step.rows * self.top
-        if self.float8 is not None:      # lists of the pairs, rows and activations in 8 bits or 32, the pairs' results; the input once more as rows
-            total += step.matrix(self.n_experts + 1, pairs, 4) + 2 * step.matrix(pairs, self.ff, 4) + step.matrix(pairs, self.hidden, 4)
+        if self.float8 is not None:      # what the experts take, and the input once more as rows
+            if step.sizes is not None:
+                total += step.sizes.experts_float8_working_bytes(step.rows, self.top, self.n_experts, self.hidden, self.ff)
             return total + 2 * step.matrix(step.rows, self.hidden) + (self.shared.working_bytes(step) if self.shared is not None else 0)
         total += step.matrix(self.n_experts, step.rows, 4) + step.matrix(pairs, self.ff) + step.matrix(pairs, self.hidden, 4)
         in_place = step.act_size == 2 and self.hidden % 64 == 0 and self.ff % 64 == 0 and self._one_launch_is_faster(pairs)
