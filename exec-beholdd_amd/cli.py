@@ -131,21 +131,20 @@ def _generate(args: list, out) -> int:
         from .cache import SequenceCache
         from .engine import open_model, parse_dtype
         from .engine.engine import GRAPH_LIMIT, entries_of_one_run
-        from .engine.memory import plan_memory
+        from .engine.memory import loaded_bytes, plan_memory
         from .kernels import KernelSizes
 
+        sizes = KernelSizes()      # the kernel library's own account of what its calls allocate: host code, no GPU is touched
         model, weights = open_model(flags["--model"], dtype, "cpu", kept_as)      # the header only: no tensor is read
         try:
-            weight_bytes = weights.planned_bytes(model.tensor_specs())
+            cache = SequenceCache(model.entry_needs, max_tokens, parse_dtype(dtype), "cpu", page, max_slots=slots,
+                                  max_position=model.max_position, banks=entries_of_one_run(model))
+            capacity = cache.n_pages * cache.page_size
+            plan = plan_memory(model, loaded_bytes(model, weights, sizes), cache.plan(), 2 if parse_dtype(dtype) == torch.bfloat16 else 4,
+                               sizes, min(step_rows or capacity, capacity), cache.max_slots, cache.max_position,
+                               page, GRAPH_LIMIT, weights=weights)
         finally:
             weights.reader.close()
-        cache = SequenceCache(model.entry_needs, max_tokens, parse_dtype(dtype), "cpu", page, max_slots=slots,
-                              max_position=model.max_position, banks=entries_of_one_run(model))
-        capacity = cache.n_pages * cache.page_size
-        # the kernel library's own account of what its calls allocate: host code, no GPU is touched
-        plan = plan_memory(model, weight_bytes, cache.plan(), 2 if parse_dtype(dtype) == torch.bfloat16 else 4,
-                           KernelSizes(), min(step_rows or capacity, capacity), cache.max_slots, cache.max_position,
-                           page, GRAPH_LIMIT)
         total = plan.total_bytes
         print(plan.describe() + (f" (budget {budget}: {'fits' if total <= budget else 'does not fit'})"
                                  if budget is not None else ""), file=out)

@@ -21,7 +21,7 @@ from ..weights.binder import bind
 from ..weights.random_init import random_tensor_on_device
 from . import generation
 from .graphs import DecodeGraphs
-from .memory import kept_logits_bytes, plan_memory
+from .memory import kept_logits_bytes, loaded_bytes, loads_in_turn, plan_memory
 from .step import StepEntry, StepError, StepStaging, build_step, cache_for_runs, check_entries
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
@@ -77,6 +77,7 @@ class Engine:
                 continue
             if isinstance(value, bool) or not isinstance(value, numbers.Integral) or value < least:
                 raise ValueError(f"{name} is an integer of at least {least}{' or None' if optional else ''}, got {value!r}")
+        sizes = kernels if hasattr(kernels, "gemm_working_bytes") else None
         with_graphs = bool(use_graphs and self.device.type == "cuda")
         if model is not None and weights != "stored":
             raise ValueError("a built model keeps its weights as it was built: weights='float8' goes with a model folder")
@@ -86,14 +87,14 @@ class Engine:
                                  max_slots=max_slots, max_position=built.max_position,
                                  banks=entries_of_one_run(built) if getattr(kernels, "state_in_banks", False) else ())
 
-        def within_budget(weight_bytes, cache):
+        def within_budget(weight_bytes, cache, bound=None):
             capacity = cache.n_pages * cache.page_size
             # never below one token for every sequence, so that a decode step of a full batch fits
             self.max_rows_per_step = min(max(int(max_rows_per_step), cache.max_slots), capacity) if max_rows_per_step else capacity
             self.plan = plan_memory(model, weight_bytes, cache.plan(), 2 if self.dtype == torch.bfloat16 else 4,
-                                    kernels if hasattr(kernels, "gemm_working_bytes") else None, self.max_rows_per_step,
+                                    sizes, self.max_rows_per_step,
                                     cache.max_slots, cache.max_position, cache.page_size, graph_limit, with_graphs,
-                                    max(int(graph_rows_per_sequence), 1))
+                                    max(int(graph_rows_per_sequence), 1), bound)
             if memory_limit_bytes is not None and self.plan.total_bytes > memory_limit_bytes:
                 raise MemoryBudgetError(f"the engine needs {self.plan.total_bytes} bytes, the limit is "
                                         f"{memory_limit_bytes}:\n{self.plan.describe()}")
@@ -108,20 +109,25 @@ class Engine:
             try:
                 if weights == "float8" and not hasattr(kernels, "pack_float8"):
                     raise ValueError("these kernels keep no weights in 8 bits")
-                self.weight_bytes = bound.planned_bytes(model.tensor_specs())
+                self.weight_bytes = loaded_bytes(model, bound, sizes)
                 self.cache = make_cache(model)
-                within_budget(self.weight_bytes, self.cache)
-                model.load(bound, self.device)
+                within_budget(self.weight_bytes, self.cache, bound)
+                if loads_in_turn(model):
+                    model.load_and_prepare(bound, self.device, kernels)
+                else:
+                    model.load(bound, self.device)
+                    if hasattr(model, "prepare"):
+                        model.prepare(kernels)
             finally:
                 bound.reader.close()
         else:
             self.weight_bytes = sum(t.numel() * t.element_size() for t in _model_tensors(model))
             self.cache = make_cache(model)
             within_budget(self.weight_bytes, self.cache)
+            if hasattr(model, "prepare"):
+                model.prepare(kernels)
         self.model = model
         self.config = model.config
-        if hasattr(model, "prepare"):
-            model.prepare(kernels)
         self.cache_plan = self.cache.allocate()
         self.sampler = Sampler(kernels, self.device, capacity=self.cache.max_slots)
         self._last_selection = None

@@ -63,25 +63,33 @@ def kept_logits_bytes(max_slots: int, vocab: int) -> int:
     return 2 * _rounded(int(max_slots) * int(vocab) * 4)
 
 
-def weights_as_kept(model, act_size: int, sizes) -> tuple:
+def weights_as_kept(model, act_size: int, sizes, weights=None) -> tuple:
     """(bytes of the weights as the engine keeps them, bytes of the largest transient while loading): a matrix
     that the kernel library regroups has its rows padded to whole blocks, and while it is stacked from its
-    checkpoint tensors or regrouped a second copy of it exists."""
+    checkpoint tensors or regrouped a second copy of it exists.  `weights`: the checkpoint's tensors, which say how many bytes those of a layer
+    take that go into 8 bits (a float32 tensor is read as float32 by every engine)."""
     kept = transient = 0
     linears = [linear for part in model.parts() for linear in _linears(part)]
     in_linears = set()
+    specs = {spec.name: spec for spec in model.tensor_specs()} if weights is not None else {}
+    for part in model.parts():
+        # a layer whose matrices go into 8 bits has all of them as stored for a while, and beside them the pieces of the matrix that is stacked, or
+        # later what bringing it into 8 bits takes
+        stored = beside = 0
+        for names, matrices, rows, cols, apart in _in_float8(part):
+            if names[0] in in_linears:
+                continue
+            element = -(-weights.planned_bytes([specs[name] for name in names]) // (matrices * rows * cols)) if weights is not None else act_size
+            kept += _in_8_bits(matrices, rows, cols, sizes)
+            stored += _rounded(matrices * rows * cols * element)
+            beside = max(beside, _rounded(apart * rows * cols * element), sizes.float8_packing_bytes(rows, cols) if sizes is not None else 0)
+            in_linears.update(names)
+        transient = max(transient, stored + beside)
     for linear in linears:
-        if getattr(linear, "shared", False):
+        if getattr(linear, "shared", False) or getattr(linear, "float8", 0):
             continue
         rows, cols = linear.out_features, linear.in_features
         packs = bool(getattr(linear, "packs", lambda size: False)(act_size))
-        if getattr(linear, "float8", 0):
-            kept += sizes.float8_bytes(linear.float8, rows // linear.float8, cols) if sizes is not None else rows * cols
-            # the stacked matrix while it is loaded; later its 8-bit form beside it, and what that takes on the way
-            transient = max(transient, _rounded(rows * cols * act_size) if len(linear.names) > 1 else 0,
-                            (sizes.float8_bytes(linear.float8, rows // linear.float8, cols) + sizes.float8_packing_bytes(rows, cols)) if sizes is not None else 0)
-            in_linears.update(linear.names)
-            continue
         size = sizes.packed_bytes(rows, cols, act_size) if (packs and sizes is not None) else _rounded(rows * cols * act_size)
         kept += size
         transient = max(transient, size if (packs or len(linear.names) > 1) else 0)
@@ -95,18 +103,48 @@ def weights_as_kept(model, act_size: int, sizes) -> tuple:
     return kept, transient
 
 
-def _linears(part, depth: int = 0) -> list:
+def loads_in_turn(model) -> bool:
+    """Whether the engine loads this model a layer at a time, each into the form that is kept (`DecoderModel.load_and_prepare`): one whose
+    layers keep matrices in 8 bits."""
+    return hasattr(model, "load_and_prepare") and any(_in_float8(part) for part in model.parts())
+
+
+def loaded_bytes(model, weights, sizes) -> int:
+    """Bytes of a model's weights once all are loaded: the checkpoint's tensors (`weights`), those that a layer brings into 8 bits as it is
+    loaded in that form."""
+    matrices = [matrix for part in model.parts() for matrix in _in_float8(part)] if loads_in_turn(model) else []
+    of = {matrix[0][0]: _in_8_bits(*matrix[1:4], sizes) for matrix in matrices}      # (a part may be found in two places)
+    gone = {name for matrix in matrices for name in matrix[0]}
+    return weights.planned_bytes([spec for spec in model.tensor_specs() if spec.name not in gone]) + sum(of.values())
+
+
+def _in_8_bits(matrices: int, rows: int, cols: int, sizes) -> int:
+    return sizes.float8_bytes(matrices, rows, cols) if sizes is not None else matrices * rows * cols
+
+
+def _linears(part) -> list:
     from ..parts.linear import Linear
-    if isinstance(part, Linear):
-        return [part]
-    found = []
+    return _found(part, lambda thing: isinstance(thing, Linear), within=False)
+
+
+def _in_float8(part) -> list:
+    """(tensor names, matrices, their rows, their columns, how many of them stand apart while they are stacked) of everything in a part that
+    is kept in 8 bits."""
+    return [matrix for thing in _found(part, lambda thing: hasattr(thing, "matrices_in_float8"), within=True) for matrix in thing.matrices_in_float8()]
+
+
+def _found(part, wanted, within: bool, depth: int = 0) -> list:
+    """What is `wanted` among a part's attributes, some levels down; `within`: also inside what is."""
+    found = [part] if wanted(part) else []
+    if found and not within:
+        return found
     if depth < 4 and hasattr(part, "__dict__"):
         for value in vars(part).values():
             if isinstance(value, (list, tuple)):
                 for item in value:
-                    found += _linears(item, depth + 1)
+                    found += _found(item, wanted, within, depth + 1)
             elif hasattr(value, "__dict__") and not isinstance(value, type):
-                found += _linears(value, depth + 1)
+                found += _found(value, wanted, within, depth + 1)
     return found
 
 
@@ -120,9 +158,11 @@ def tables_bytes(model) -> int:
 
 
 def plan_memory(model, weight_bytes: int, cache_plan, act_size: int, sizes, max_rows_per_step: int, max_slots: int,
-                max_position: int, page_size: int, graph_limit: int, graphs: bool = True, graph_rows: int = 1) -> MemoryPlan:
+                max_position: int, page_size: int, graph_limit: int, graphs: bool = True, graph_rows: int = 1, weights=None) -> MemoryPlan:
+    """`weight_bytes`: what the weights take once they are loaded (`loaded_bytes`); `weights`: the checkpoint's tensors, of a model that is
+    loaded from one."""
     plan = MemoryPlan()
-    kept, transient = weights_as_kept(model, act_size, sizes)
+    kept, transient = weights_as_kept(model, act_size, sizes, weights)
     plan.add("weights", int(weight_bytes))
     plan.add("weights' padding to the kernels' blocks and the allocator's units", max(kept - int(weight_bytes), 0))
     plan.add("largest transient while the weights are loaded and regrouped", transient)

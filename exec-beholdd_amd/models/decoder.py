@@ -109,6 +109,21 @@ class DecoderModel:
             if hasattr(part, "prepare"):
                 part.prepare(kernels)
 
+    def load_and_prepare(self, get, device, kernels):
+        """`load` and `prepare` a layer at a time: a layer's matrices are in the form that is kept before the next layer's are read, so that no
+        more than one layer is in the device's memory as it is stored."""
+        blocks = {id(block) for block in self.own_blocks()}
+        for part in self.parts():
+            part.load(get)
+            if id(part) in blocks and hasattr(part, "prepare"):
+                part.prepare(kernels)
+        for part in self.shared_parts:
+            if hasattr(part, "build_tables"):
+                part.build_tables(device)
+        for part in self.parts():
+            if id(part) not in blocks and hasattr(part, "prepare"):
+                part.prepare(kernels)
+
     def working_bytes(self, step) -> int:
         """Bytes a step of these sizes allocates at its peak: the residual, the widest layer (a layer's
         temporaries are freed before the next one runs; what a block prepares for the next is counted with

@@ -49,7 +49,8 @@ step is launched kernel by kernel or replayed from a capture, so a state advance
 Every part may say what its forward allocates: working_bytes(step: StepSize) -> int, from sizes alone; the
 engine's byte plan adds them up before anything is allocated and names the parts that do not say.
 A part whose matrices may be kept in 8 bits offers keep_in_float8(): called before anything is loaded or planned, it has `prepare`
-keep them so (`Linear.keep_in_float8`).  Parts that do not offer it keep theirs as they are.
+keep them so (`Linear.keep_in_float8`), and matrices_in_float8() for the byte plan where these are not `Linear`s among its attributes.
+An engine then loads and prepares the model a layer at a time.  Parts that do not offer it keep theirs as they are.
 A part may declare `graph_safe = True`: its forward uses only the device tensors of the step
 context (never the host_* lists, never a host-side decision that changes from step to step).
 Decode steps of a model whose parts all say so are captured and replayed as HIP graphs.  That speaks of steps

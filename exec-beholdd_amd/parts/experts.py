@@ -167,6 +167,13 @@ class RoutedExperts:
         if hasattr(self.shared, "keep_in_float8"):
             self.shared.keep_in_float8()
 
+    def matrices_in_float8(self) -> list:
+        """The stacks that `prepare` keeps in 8 bits, as `Linear.matrices_in_float8` has them; `load` holds the first expert's gate and one more."""
+        if self.float8 is None:
+            return []
+        names = lambda *kinds: [f"{self.prefix}e{e}.{kind}" for e in range(self.n_experts) for kind in kinds]
+        return [(names("gate", "up"), 2 * self.n_experts, self.ff, self.hidden, 2), (names("down"), self.n_experts, self.hidden, self.ff, 2)]
+
     def prepare(self, kernels):
         """The stacked matrices stay row after row (the kernels for steps of few rows read them so).  For prompts every expert's
         matrices are kept a second time in the kernel library's own form, where it has one for them: its products of many rows
@@ -181,9 +188,10 @@ class RoutedExperts:
         if self.shared is not None:
             self.shared.prepare(kernels)
         if self.float8 is not None:
-            self.float8 = (kernels.pack_float8(self.w_gate_up.view(-1, self.hidden), matrices=2 * self.n_experts),
-                           kernels.pack_float8(self.w_down.view(-1, self.ff), matrices=self.n_experts))
-            self.w_gate_up = self.w_down = None
+            up = kernels.pack_float8(self.w_gate_up.view(-1, self.hidden), matrices=2 * self.n_experts)
+            self.w_gate_up = None
+            self.float8 = (up, kernels.pack_float8(self.w_down.view(-1, self.ff), matrices=self.n_experts))
+            self.w_down = None
             return
         tiles = getattr(kernels, "experts_tiles_take", None)
         if tiles is not None and tiles(self.w_gate_up.dtype, self.hidden, self.ff) and tiles(self.w_down.dtype, self.ff, self.hidden):

@@ -62,6 +62,13 @@ class Linear:
             raise ValueError(f"{self.out_features} rows are not those of {matrices} equal matrices")
         self.float8 = int(matrices)
 
+    def matrices_in_float8(self) -> list:
+        """What `prepare` keeps in 8 bits, for the byte plan: [(tensor names, matrices, their rows, their columns, how many of them stand apart
+        while `load` stacks them)]."""
+        if not self.float8 or self.shared:
+            return []
+        return [(self.names, self.float8, self.out_features // self.float8, self.in_features, self.float8 if len(self.names) > 1 or self.padding else 0)]
+
     def reader(self, swiglu: bool = False) -> ProductReader:
         """This map as the only reader of an activation matrix (`swiglu`: its rows are gate rows, then up rows)."""
         return ProductReader(self.out_features // 2 if swiglu else self.out_features, swiglu,

@@ -45,6 +45,10 @@ class TimeMixing:
     def _linears(self):
         return [*self.projections.values(), self.decay_down, self.decay_up, self.out]
 
+    def matrices_in_float8(self) -> list:
+        """(Those of the output are its own to name.)"""
+        return [matrix for linear in self.projections.values() for matrix in linear.matrices_in_float8()]
+
     def keep_in_float8(self):
         for linear in (*self.projections.values(), self.out):
             linear.keep_in_float8()
