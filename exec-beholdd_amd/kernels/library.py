@@ -1021,6 +1021,8 @@ class HipKernels(KernelSizes):
         return (values[:, :w.rows, :cols].contiguous().view(torch.float8_e4m3fn).to(torch.float32) * spread).reshape(total, cols)
 
     def _new_float8_rows(self, rows, width, in_rows) -> Float8Rows:
+        if rows < 1 or width < 1:
+            raise KernelError(f"rows in 8 bits: at least one row of one value, got {rows} x {width}")
         (data_bytes, exponent_bytes), words = Float8Rows.bytes_of(rows, width), -(-width // 512)
         return Float8Rows(torch.empty(data_bytes, dtype=torch.uint8, device=self.device),
                           torch.empty((words, exponent_bytes // 4 // words), dtype=torch.int32, device=self.device), rows, width, in_rows)
