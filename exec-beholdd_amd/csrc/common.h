@@ -91,6 +91,9 @@ inline void bh_wide_row(int n_rows, int pieces, int* threads, int* per) {
 }
 
 // ---- gated activations ----------------------------------------------------------------------
+// A value held to a limit, or between its negative and itself.  A NaN stays one, so that a broken row shows (fminf and fmaxf would give the limit).
+__device__ inline float held_below(float v, float limit) { return v > limit ? limit : v; }
+__device__ inline float held_between(float v, float limit) { return held_below(v < -limit ? -limit : v, limit); }
 // act(gate) * up with act(g) = g / (1 + exp(-g (slope + cube g^2))): silu with slope 1 and cube 0, and with slope
 // 2 sqrt(2/pi) and cube 2 sqrt(2/pi) 0.044715 the tanh form of GELU, since (1 + tanh(y)) / 2 = 1 / (1 + exp(-2y)).
 // `squared`: no gate, but max(x, 0)^2 on a plain product's bfloat16 output.
@@ -112,8 +115,8 @@ __device__ inline float relu_squared(float x) {
 template <bool CLAMPED = false>
 __device__ inline float gate_mul(float gate, float up, GateForm form) {
   if constexpr (CLAMPED) {
-    gate = fminf(gate, form.cube);
-    return gate / (1.0f + expf(-gate * form.slope)) * (fminf(fmaxf(up, -form.cube), form.cube) + 1.0f);
+    gate = held_below(gate, form.cube);
+    return gate / (1.0f + expf(-gate * form.slope)) * (held_between(up, form.cube) + 1.0f);
   }
   return gate / (1.0f + expf(-gate * fmaf(form.cube, gate * gate, form.slope))) * up;
 }

@@ -16,8 +16,8 @@
 #include "common.h"
 
 __device__ inline float clamped_glu(float g, float u, float limit, float alpha, float shift) {
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = held_below(g, limit);
+  u = held_between(u, limit);
   return g / (1.0f + expf(-alpha * g)) * (u + shift);
 }
 

@@ -19,8 +19,8 @@ struct ExpertGate {
   float limit, alpha, shift;
 };
 __device__ inline float activated(float g, float u, const ExpertGate& gate) {
-  g = g > gate.limit ? gate.limit : g;      // (fminf and fmaxf would give the limit for a NaN)
-  u = u > gate.limit ? gate.limit : u < -gate.limit ? -gate.limit : u;
+  g = held_below(g, gate.limit);
+  u = held_between(u, gate.limit);
   return f8_gated(g, gate.alpha * g) * (u + gate.shift);
 }
 

@@ -32,8 +32,8 @@ namespace {
 __device__ inline xm_bf16x8_t as_operand(xm_u32x4_t v) { return __builtin_bit_cast(xm_bf16x8_t, v); }
 
 __device__ inline float activation(float g, float u, float limit, float alpha, float shift) {
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = held_below(g, limit);
+  u = held_between(u, limit);
   return g / (1.0f + expf(-alpha * g)) * (u + shift);
 }
 

@@ -29,8 +29,8 @@ __device__ inline em_bf16x8_t em_operand(const uint16_t* p) {
 }
 
 __device__ inline float em_act(float g, float u, float limit, float alpha, float shift) {
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = held_below(g, limit);
+  u = held_between(u, limit);
   return g / (1.0f + expf(-alpha * g)) * (u + shift);
 }
 

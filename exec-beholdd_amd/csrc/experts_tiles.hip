@@ -87,7 +87,7 @@ __global__ __launch_bounds__(WAVES * BH_WAVE) void experts_tiles_kernel(const ui
       const size_t at = (size_t)pair * N + n;
       if (GATED) {
         const float weight = in_weights ? in_weights[pair] : 1.0f;
-        const float gate = fminf(sum[0] * weight, limit), up = fminf(fmaxf(sum[SIDES - 1] * weight, -limit), limit);
+        const float gate = held_below(sum[0] * weight, limit), up = held_between(sum[SIDES - 1] * weight, limit);
         reinterpret_cast<bf16_t*>(out_raw)[at] = from_f32<bf16_t>(gate / (1.0f + expf(-alpha * gate)) * (up + shift));
       } else {
         reinterpret_cast<float*>(out_raw)[at] = sum[0];
