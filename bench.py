@@ -45,6 +45,7 @@ def parse():
     parser.add_argument("--context", type=int, default=8192)
     parser.add_argument("--prefill-tokens", type=int, default=2048)
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--weights", default="stored", choices=["stored", "float8"], help="how the layers' matrices are kept (with --shape only)")
     parser.add_argument("--no-points", action="store_true", help="skip the batch 1 and 64 decode points")
     parser.add_argument("--workload", action="store_true",
                         help="instead of the step timings, generate through the engine's own loop for the batch the shape's "
@@ -1420,7 +1421,7 @@ def main():
     device = "cuda:0"
     dtype_tag = "bf16" if args.dtype == "bfloat16" else "fp32"
     element = 2 if args.dtype == "bfloat16" else 4
-    model = random_model_on_device(config, seed=0, dtype=args.dtype, device=device)
+    model = random_model_on_device(config, seed=0, dtype=args.dtype, device=device, weights=args.weights)
     biggest = 1 if args.no_points else 64
     if args.workload:
         count, _, longest, new_tokens, _, context = WORKLOADS[args.shape]
@@ -1440,7 +1441,8 @@ def main():
 
     layer_params = (cfg.hidden * (cfg.q_width + 2 * cfg.kv_width) + cfg.q_width * cfg.hidden
                     + 3 * cfg.hidden * cfg.intermediate)
-    weight_bytes = (cfg.n_layers * layer_params + cfg.vocab * cfg.hidden) * element
+    layer_bytes = cfg.n_layers * layer_params * (element if args.weights == "stored" else 1 + 4 / 128 ** 2)      # (a float32 scale for each 128 x 128)
+    weight_bytes = layer_bytes + cfg.vocab * cfg.hidden * element
     kv_bytes_per_token = cfg.n_layers * 2 * cfg.kv_width * element
 
     seconds, mean_length = decode_run(engine, args.batch, args.context, args.steps, args.warmup, torch)
@@ -1516,11 +1518,13 @@ def main():
         "points": points,
         "points_hbm_frac": fractions,
     }
+    if args.weights != "stored":
+        line["config"]["weights"] = args.weights
     if prefill_points:
         line["prefill_points"] = prefill_points
     if generated is not None:
         line["generate"] = generated
-    if not args.no_points and args.shape == "8b" and args.layers is None and args.dtype == "bfloat16":
+    if not args.no_points and args.shape == "8b" and args.layers is None and args.dtype == "bfloat16" and args.weights == "stored":
         # the other two shapes of the family, full depth: decode at batch 8 and the prompt of 2,048 tokens
         del engine, model, cache_tensor, span
         line["shapes"] = {name: other_shape(name, args, torch) for name in ("14b", "32b")}

@@ -57,8 +57,11 @@ class Engine:
     crates/beholdd-model/src/qwen3moe/recorded_attention.rs:344-365).
     `weights="float8"` keeps the matrices of the layers in 8-bit floating point with a scale for each block of 128 x 128, made from the
     checkpoint's as it is loaded, and brings the rows that are multiplied with them into 8 bits too, a scale for each 128 values; the embedding,
-    the head, routers, norms and small tables stay as they are.  Half the bytes of bfloat16 to keep and to read in every step, at results that
-    differ from the stored weights' by the roundings to 8 bits (2^-4 of a value at most)."""
+    the head, routers, norms and small tables stay as they are.  Half the bytes of bfloat16 to keep and to read in every step, and one layer as it is
+    stored beside them while the model loads.  Results differ from the stored weights' by the roundings to 8 bits: half a step of e4m3 each, which is
+    2^-4 of a value at most, or 2^-10 of its scale where that is more (values below a 28,672nd of what the scale can hold, the smallest of
+    which become zero).  A float32 engine adds the products up in float32; a bfloat16 engine as the 8-bit matrix cores do, into the float32
+    residual too (1.4e-5 of a sum by norm, 2^-9 of what comes from bfloat16 activations), but the gates and ups of routed experts in float32."""
 
     def __init__(self, model_dir: str | None = None, dtype="bfloat16", max_tokens: int = 4096,
                  max_slots: int | None = None, device="cuda:0", kernels=None, model=None,
@@ -296,12 +299,15 @@ def load_model(model_dir: str, dtype, device):
     return model
 
 
-def random_model_on_device(config_dict: dict, seed: int, dtype, device):
-    """A model with seeded random weights drawn on the device (nothing is written to disk)."""
+def random_model_on_device(config_dict: dict, seed: int, dtype, device, weights: str = "stored"):
+    """A model with seeded random weights drawn on the device (nothing is written to disk).  `weights`: as an engine will keep the layers'
+    matrices ("stored", or "float8" once it has prepared them)."""
     dtype = parse_dtype(dtype)
     entry = resolve_architecture(config_dict)
     config = configuration_of(entry, config_dict)
     model = entry.build(config)
+    if weights == "float8":
+        model.keep_in_float8()
     specs = {spec.name: spec for spec in model.tensor_specs()}
     model.load(lambda name: random_tensor_on_device(specs[name], seed, device, dtype), device)
     return model

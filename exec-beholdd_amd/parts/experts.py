@@ -18,7 +18,8 @@ neighbouring experts only, judged by their best expert or the sum of their two b
 + correction with scores of either kind ("sigmoid" or "softmax_all"), the chosen scores are divided by their sum with `renorm`, and multiplied
 by `factor` (`kernels.route_in_groups`).
 
-With `keep_in_float8()` the experts' matrices are kept in 8 bits alone, and all of a step's pairs go through `kernels.experts_float8`.
+With `keep_in_float8()` the experts' matrices are kept in 8 bits alone, and all of a step's pairs go through `kernels.experts_float8`, whose gate and up
+sums are float32's and whose last product adds up as the engine's others do (`Linear`).
 
 The experts' matrices are kept stacked: gate and up rows of an expert in one [2 ff, width] block, [experts, ...] in
 all.  The (row, choice) pairs are grouped by expert on the device (`experts_group`).  A step of few rows then runs a
